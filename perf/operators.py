@@ -253,7 +253,7 @@ def _linear(s):
     else:
         big = x.abs().amax(1)
         xs = big / 127
-        x = torch.round(x * (127 / big)[:, None])
+        x = torch.round(x * (torch.full_like(big, 127) / big)[:, None])  # (a number / tensor is its reciprocal times it)
     y = (x @ s["w"].float().t()) * (xs[:, None] * s["ws"][None, :])
     if s["b"] is not None:
         y = y + s["b"].float()
@@ -375,7 +375,7 @@ def _exact_linear(case, s):
         xs = s["xs"].double()
     else:
         big = s["x"].float().abs().amax(1, keepdim=True)
-        x = torch.round(s["x"].float() * (127 / big)).double()
+        x = torch.round(s["x"].float() * (torch.full_like(big, 127) / big)).double()
         xs = big[:, 0].double() / 127
     y = torch.einsum("mk,nk->mn", x, s["w"].double()).mul_(xs[:, None]).mul_(s["ws"].double()[None])
     if s["b"] is not None:
