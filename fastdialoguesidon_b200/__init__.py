@@ -12,6 +12,11 @@ Public API (mirrors the attention ops of ``fds_triton.kernels``):
   either side of the attention (QKV with bias, the DiT's QKV with RoPE in the
   epilogue, the out-projection accumulated into the fp32 residual), and
   :func:`rotated_attention` for the DiT attention over a pre-rotated qkv;
+- :func:`window_attention`: attention over a sliding window of keys with sinks
+  (long recordings, streams);
+- :func:`quantize_rows`, :func:`linear_int8`, :func:`linear_int8_rope`,
+  :func:`accumulate_int8`: the projections in 8-bit integers;
+- :func:`residual_norm`: the norms, gate and residual scale between two blocks;
 - :func:`check_status`: raise if a kernel reported a bounded-wait timeout.
 
 The same ops are registered as ``torch.ops.fds.flexrel_attention`` and
@@ -37,6 +42,14 @@ from .kernels import (  # noqa: F401
     rope_split,
     rope_tables,
     rotated_attention,
+)
+from .layer_ops import (  # noqa: F401
+    accumulate_int8,
+    linear_int8,
+    linear_int8_rope,
+    quantize_rows,
+    residual_norm,
+    window_attention,
 )
 from . import torch_ops  # noqa: F401  (registers torch.ops.fds.*)
 

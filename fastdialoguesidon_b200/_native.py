@@ -36,8 +36,11 @@ FDS_EPILOGUE_ACCUMULATE_F32 = 2
 FDS_GEMM_AUTO = 0
 FDS_GEMM_SINGLE = 1
 FDS_GEMM_PAIR = 2
+FDS_NORM_NONE = 0
+FDS_NORM_LAYER = 1
+FDS_NORM_RMS = 2
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # every symbol include/fds_b200.h declares (checked by the CPU test suite)
 EXPORTED_SYMBOLS = (
@@ -52,6 +55,9 @@ EXPORTED_SYMBOLS = (
     "fds_attn_schedule",
     "fds_linear_fwd",
     "fds_flexrel_qr_attn_fwd",
+    "fds_linear_int8_fwd",
+    "fds_residual_norm_fwd",
+    "fds_window_attn_fwd",
 )
 
 
@@ -156,6 +162,96 @@ class FdsLinearArgs(ctypes.Structure):
     ]
 
 
+class FdsLinearInt8Args(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("a_row_stride", ctypes.c_int64),
+        ("a_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_row_stride", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("status_host", ctypes.c_void_p),
+        ("m", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("epilogue", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("rope_cols", ctypes.c_int32),
+        ("timeout_ns", ctypes.c_int64),
+        ("tile_n", ctypes.c_int32),
+        ("cta_pair", ctypes.c_int32),
+    ]
+
+
+class FdsResidualNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("x_out", ctypes.c_void_p),
+        ("x_out_stride", ctypes.c_int64),
+        ("h", ctypes.c_void_p),
+        ("h_stride", ctypes.c_int64),
+        ("h_scale", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("gate_stride", ctypes.c_int64),
+        ("post_w", ctypes.c_void_p),
+        ("post_b", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("shift", ctypes.c_void_p),
+        ("mod_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("c", ctypes.c_int32),
+        ("length", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("x_f32", ctypes.c_int32),
+        ("param_f32", ctypes.c_int32),
+        ("post", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("alpha", ctypes.c_float),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class FdsWindowArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("out_stride", ctypes.c_int64 * 3),
+        ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("status_host", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("q_len", ctypes.c_int32),
+        ("k_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("left", ctypes.c_int32),
+        ("right", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("timeout_ns", ctypes.c_int64),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -188,6 +284,12 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fds_flexrel_qr_attn_fwd.restype = ctypes.c_int
         lib.fds_linear_fwd.argtypes = [ctypes.POINTER(FdsLinearArgs), ctypes.c_void_p]
         lib.fds_linear_fwd.restype = ctypes.c_int
+        for name, struct in (("fds_linear_int8_fwd", FdsLinearInt8Args),
+                             ("fds_residual_norm_fwd", FdsResidualNormArgs),
+                             ("fds_window_attn_fwd", FdsWindowArgs)):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+            fn.restype = ctypes.c_int
         lib.fds_rope_split.argtypes = [
             ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
             ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,

@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -21,7 +22,7 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libfds_b200.so"
 INCLUDE_DIR = REPO_DIR / "include"
 
-SOURCES = ["fds_capi.cu", "fds_rope_static.cu"]
+SOURCES = ["fds_capi.cu", "fds_rope_static.cu", "fds_int8.cu", "fds_norm.cu", "fds_window.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 # The attention kernels split their register file with setmaxnreg
@@ -32,6 +33,9 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # refuses to produce a library in that case.
 ATTN_KERNEL_MARK = "attn_fwd_kernel"
 ATTN_LAUNCH_REGS = 168
+# ... and of the window kernel (csrc/window_kernel.cuh: 128 threads at 208, 128 at 48)
+WINDOW_KERNEL_MARK = "window_tile_kernel"
+WINDOW_LAUNCH_REGS = 128
 
 
 def nvcc_path() -> str:
@@ -55,47 +59,58 @@ def is_stale() -> bool:
     return any(f.stat().st_mtime > mtime for f in _inputs())
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if any source is newer than it (or ``force``)."""
-    if not force and not is_stale():
-        return LIB_PATH
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [
-        nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xptxas=-v",
-        "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
-        "-I", str(INCLUDE_DIR),
-        "-o", str(tmp),
-        *[str(CSRC / s) for s in SOURCES],
-    ]
+def _run(cmd: list[str], verbose: bool) -> str:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    return res.stdout + res.stderr
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the library if any source is newer than it (or ``force``)."""
+    if not force and not is_stale():
+        return LIB_PATH
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    # the sources compile side by side, each to an object, then link
+    objs = [LIB_DIR / (Path(src).stem + ".o") for src in SOURCES]
+
+    def compile_one(job: tuple[str, Path]) -> str:
+        src, obj = job
+        return _run([nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xptxas=-v", "-Xcompiler",
+                     "-fPIC,-fvisibility=hidden", "-I", str(INCLUDE_DIR), "-c", "-o", str(obj), str(CSRC / src)], verbose)
+
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+        log = "".join(pool.map(compile_one, zip(SOURCES, objs)))
+    tmp = LIB_PATH.with_suffix(".so.tmp")
+    _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(tmp), *map(str, objs)], verbose)
+    for obj in objs:
+        obj.unlink()
     if verbose:
-        sys.stdout.write(res.stdout + res.stderr)
-    check_launch_registers(res.stdout + res.stderr)
+        sys.stdout.write(log)
+    check_launch_registers(log)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 
 
 def check_launch_registers(ptxas_log: str) -> None:
-    """Every attention kernel entry must report ATTN_LAUNCH_REGS registers."""
-    current, seen = None, 0
-    for line in ptxas_log.splitlines():
-        if "Compiling entry function" in line:
-            current = line
-        elif current and "Used" in line and "registers" in line:
-            if ATTN_KERNEL_MARK in current:
-                regs = int(line.split("Used")[1].split("registers")[0])
-                if regs != ATTN_LAUNCH_REGS:
-                    raise RuntimeError(f"attention kernel launches with {regs} registers per thread, expected "
-                                       f"{ATTN_LAUNCH_REGS} (the setmaxnreg split depends on it): {current}")
-                seen += 1
-            current = None
-    if seen == 0:
-        raise RuntimeError("no attention kernel found in the ptxas report")
+    """Every kernel that splits its registers must launch with the count its split assumes."""
+    for mark, expected in ((ATTN_KERNEL_MARK, ATTN_LAUNCH_REGS), (WINDOW_KERNEL_MARK, WINDOW_LAUNCH_REGS)):
+        current, seen = None, 0
+        for line in ptxas_log.splitlines():
+            if "Compiling entry function" in line:
+                current = line
+            elif current and "Used" in line and "registers" in line:
+                if mark in current:
+                    regs = int(line.split("Used")[1].split("registers")[0])
+                    if regs != expected:
+                        raise RuntimeError(f"attention kernel launches with {regs} registers per thread, expected "
+                                           f"{expected} (the setmaxnreg split depends on it): {current}")
+                    seen += 1
+                current = None
+        if seen == 0:
+            raise RuntimeError(f"no {mark} found in the ptxas report")
 
 
 if __name__ == "__main__":

@@ -620,7 +620,7 @@ __device__ __forceinline__ constexpr bool poly_pair(int c) {
 // O *= alpha for this thread's row (32 lanes of a warp, 64 columns). Rare (the
 // running max moves by more than the lazy threshold), so it is kept out of line:
 // its registers then never compete with the exponentials of the hot loop.
-__device__ __noinline__ void rescale_o_row(uint32_t tO, float alpha) {
+inline __device__ __noinline__ void rescale_o_row(uint32_t tO, float alpha) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         uint32_t o[32];
@@ -630,6 +630,15 @@ __device__ __noinline__ void rescale_o_row(uint32_t tO, float alpha) {
         for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
         tmem_st32(tO + 32 * half, o);
     }
+}
+
+// Which keys of a tile a step excludes: none, those from kv_end on, or (window
+// attention, window_kernel.cuh) all but two ranges of the row's own.
+enum MaskKind : int { kMaskNone = 0, kMaskTail = 1, kMaskWindow = 2 };
+
+// The n lowest bits of a word (n clamped to [0, 32]).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
 }
 
 // Online softmax of one query row (this thread) over the KV tiles: per tile,
@@ -646,11 +655,13 @@ struct RowSoftmax {
     int i, kv_end, lane, t_begin;
     float m_run, l_run;
     uint32_t s_parity, pv_parity;
+    int w_first, w_lo, w_hi;  // kMaskWindow: columns c < w_first and w_lo <= c < w_hi of the tile are seen
 
     // kBand: per-score relative bias gathered from qrow (any tile; needed for
     // the near-diagonal ones); otherwise the per-row constant cb (a tile whose
-    // every pair saturates the clamp, or no bias). kMask: keys >= kv_end.
-    template <bool kBand, bool kMask>
+    // every pair saturates the clamp, or no bias). kMask: the keys excluded
+    // (MaskKind). A row that has seen no key yet keeps m_run = -inf, l_run = 0.
+    template <bool kBand, int kMask>
     __device__ __forceinline__ bool step(int j, float cb) {
         bool ok = warp_wait(s_full, s_parity, ctl, err);
         s_parity ^= 1;
@@ -687,7 +698,16 @@ struct RowSoftmax {
             mult = 1.f;
             cb = 0.f;
         }
-        if constexpr (kMask) {
+        if constexpr (kMask == kMaskWindow) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t seen = low_bits(w_first - 32 * k) | (low_bits(w_hi - 32 * k) & ~low_bits(w_lo - 32 * k));
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    if ((seen & (1u << c)) == 0) s[32 * k + c] = -INFINITY;
+            }
+        }
+        if constexpr (kMask == kMaskTail) {
             const int lim = kv_end - n0;
 #pragma unroll
             for (int c = 0; c < 128; ++c)
@@ -713,7 +733,8 @@ struct RowSoftmax {
             alpha = ex2_approx(m_run - tile_max);  // 0 on the item's first tile
             m_run = tile_max;
         }
-        const float add = cb - m_run;
+        // (a row whose every key so far is excluded: 0, so that its exponentials are 0)
+        const float add = kMask == kMaskWindow && m_run == -INFINITY ? 0.f : cb - m_run;
         const float ky = mult * (1.0f / kPolySpan), kb = (add - kPolyLo) * (1.0f / kPolySpan);
 
         // exponentials into packed 16-bit pairs, held in registers; some pairs
@@ -748,7 +769,7 @@ struct RowSoftmax {
                 warp_arrive(p_half, lane);
             }
             float2 pp;
-            if (poly_pair<kRelBias>(c)) {
+            if (kMask != kMaskWindow && poly_pair<kRelBias>(c)) {  // (the polynomial is > 0 at -inf)
                 pp = exp2_poly2(s[2 * c], s[2 * c + 1], ky, kb);
             } else {
                 const float2 x = ffma2(make_float2(s[2 * c], s[2 * c + 1]), mult2, add2);
@@ -1024,13 +1045,13 @@ __device__ __forceinline__ void softmax_role(uint32_t sbase, uint32_t tmem, cons
             const int t0 = it.q_base + wg * kBlockM;
             const int jb0 = t0 >= 190 ? (t0 - 190 + kBlockN - 1) / kBlockN : 0;
             const int jb1 = (t0 + 135 + kBlockN - 1) / kBlockN;
-            for (; ok && j < min(jb0, j_last); ++j) ok = rs.template step<false, false>(j, qr_left);
-            for (; ok && j < min(jb1, j_last); ++j) ok = rs.template step<true, false>(j, 0.f);
-            for (; ok && j < j_last; ++j) ok = rs.template step<false, false>(j, qr_right);
-            if (ok) ok = rs.template step<true, true>(j_last, 0.f);
+            for (; ok && j < min(jb0, j_last); ++j) ok = rs.template step<false, kMaskNone>(j, qr_left);
+            for (; ok && j < min(jb1, j_last); ++j) ok = rs.template step<true, kMaskNone>(j, 0.f);
+            for (; ok && j < j_last; ++j) ok = rs.template step<false, kMaskNone>(j, qr_right);
+            if (ok) ok = rs.template step<true, kMaskTail>(j_last, 0.f);
         } else {
-            for (; ok && j < j_last; ++j) ok = rs.template step<false, false>(j, 0.f);
-            if (ok) ok = rs.template step<false, true>(j_last, 0.f);
+            for (; ok && j < j_last; ++j) ok = rs.template step<false, kMaskNone>(j, 0.f);
+            if (ok) ok = rs.template step<false, kMaskTail>(j_last, 0.f);
         }
         if (!ok) break;
 

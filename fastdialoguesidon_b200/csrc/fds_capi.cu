@@ -21,6 +21,8 @@
 #include "gemm_kernel.cuh"
 #include "rope.cuh"
 
+using namespace fds_detail;
+
 namespace {
 
 thread_local std::string g_last_error;
@@ -39,48 +41,6 @@ int ok() {
     g_last_error.clear();
     return FDS_OK;
 }
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(f);
-    });
-    return fn;
-}
-
-// Device must be compute capability 10.0 (B200 / sm_100a). Cached per device;
-// the entries are atomics so that first calls from several host threads do not
-// race (every thread computes the same value).
-int check_device() {
-    static std::atomic<int> cached[64];  // 0 unknown, 1 ok, 2 unsupported
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return fail(FDS_ERR_CUDA, "cudaGetDevice: %s", cudaGetErrorString(e));
-    if (dev < 0 || dev >= 64) return fail(FDS_ERR_UNSUPPORTED_DEVICE, "device index %d out of range", dev);
-    int state = cached[dev].load(std::memory_order_relaxed);
-    if (state == 0) {
-        int major = 0, minor = 0;
-        cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-        cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-        state = (major == 10 && minor == 0) ? 1 : 2;
-        cached[dev].store(state, std::memory_order_relaxed);
-    }
-    if (state != 1)
-        return fail(FDS_ERR_UNSUPPORTED_DEVICE, "device %d is not sm_100 (B200); this library is built for sm_100a",
-                    dev);
-    return FDS_OK;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // 3-D map over a [batch, seq_len, width] view of rows with `row_stride` elements:
 // box = 64 columns x `box_rows` rows x 1 window, 128-byte swizzle, zero fill
@@ -176,63 +136,6 @@ int make_rope_table_map(CUtensorMap* map, const float* base, int64_t seq_len) {
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(FDS_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled(rope table) failed (%d)", static_cast<int>(r));
     return FDS_OK;
-}
-
-// Kernels are launched with programmatic stream serialization: a launch may
-// start its CTAs while the previous kernel in the stream drains, and waits in
-// the kernel (griddepcontrol.wait) before touching memory. FDS_PDL=0 in the
-// environment turns this off (plain stream order).
-bool pdl_enabled() {
-    static const bool on = [] {
-        const char* v = std::getenv("FDS_PDL");
-        return v == nullptr || std::strcmp(v, "0") != 0;
-    }();
-    return on;
-}
-
-// cudaFuncSetAttribute(kern, MaxDynamicSharedMemorySize, bytes) once per
-// kernel and device (it is per-device state, and a per-call driver round trip
-// otherwise); `done` is the kernel's own set of devices already configured.
-template <typename Kern>
-cudaError_t set_smem_once(Kern kern, int bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = dev >= 0 && dev < 64 ? (uint64_t{1} << dev) : 0;
-    if (bit != 0 && (done.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && bit != 0) done.fetch_or(bit, std::memory_order_release);
-    return e;
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                       Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
-// SMs of the current device (cached per device, atomically as above); 0 if it
-// cannot be queried.
-int sm_count() {
-    static std::atomic<int> cached[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    int n = cached[dev].load(std::memory_order_relaxed);
-    if (n == 0) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        cached[dev].store(n, std::memory_order_relaxed);
-    }
-    return n;
 }
 
 // Workspace of the split last wave for up to G pieces: the part counts (one
@@ -366,28 +269,9 @@ int fds_detail::set_error(int code, const char* fmt, ...) {
     return code;
 }
 
-namespace {
+int fds_detail::set_ok() { return ok(); }
 
-// Clusters of two CTAs (the pair GEMM), with PDL like launch_pdl.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pair(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                        Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
+namespace {
 
 // The linear layers' tensor maps: A, W, the output, and the RoPE epilogue's
 // cos / sin tables (copies of the output map for the other epilogues).

@@ -9,6 +9,10 @@
 //            rotated straight from the GEMM output)
 //   kAccum   out (fp32) += D (+ bias)                        (x += a W^T into
 //            the fp32 residual stream, torch.addmm(out_dtype=fp32, out=x))
+// A and W are fp16 / bf16, or (kInt8) 8-bit integers with one fp32 scale per
+// row of A (token) and per row of W (output channel): the tensor cores sum the
+// products exactly in 32-bit integers (|sum| <= 127^2 K < 2^31 for K <= 2^17)
+// and the epilogues read D[m, n] = sum * (a_scale[m] * w_scale[n]).
 //
 // Persistent CTAs, one per SM at most, walk the output tiles in a static
 // stride: 128 x BN tiles, one per CTA, or (kPair) 256 x BN tiles over a
@@ -44,7 +48,9 @@ namespace fds {
 namespace gemm {
 
 constexpr int kBM = 128;
-constexpr int kBK = 64;
+constexpr int kBK = 64;            // K elements of a stage; 8-bit operands: kBK8
+constexpr int kBK8 = 128;
+constexpr int kRowBytes = 128;     // bytes of a staged operand row (either width)
 constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4;
 constexpr int kEpiWarps = 8;
@@ -59,8 +65,8 @@ enum Epi : int { kStore = 0, kRope = 1, kAccum = 2 };
 template <int BN, bool kPair, bool kCs = false>
 struct Smem {
     static constexpr int kBNc = kPair ? BN / 2 : BN;  // W rows this CTA loads per tile
-    static constexpr int a_bytes = kBM * kBK * 2;
-    static constexpr int b_bytes = kBNc * kBK * 2;
+    static constexpr int a_bytes = kBM * kRowBytes;
+    static constexpr int b_bytes = kBNc * kRowBytes;
     static constexpr int kCsBytes = kCs ? 2 * kBM * 128 : 0;
     static constexpr int kStages = (192 * 1024 - kCsBytes) / (a_bytes + b_bytes);
     static constexpr int a = 0;
@@ -91,13 +97,15 @@ struct Params {
     const void* bias;         // [N] operand type, or null
     const float* cos_t;       // kRope: fp32 [>= seq_len, 64]
     const float* sin_t;
+    const float* a_scale;     // kInt8: [M]
+    const float* w_scale;     // kInt8: [N]
     int32_t* status;
     int32_t* status_host;
     int64_t timeout_ns;
     int32_t m, n, k;
     int32_t seq_len;          // kRope: position = row % seq_len
     int32_t rope_cols;        // kRope: columns [0, rope_cols) are rotated
-    int32_t tiles_n;          // N / BN
+    int32_t tiles_n;          // ceil(N / BN)
     int32_t tiles;            // ceil(M / tile rows) * tiles_n
 };
 
@@ -130,6 +138,30 @@ __device__ __forceinline__ float bias_at(const uint4 (&raw)[4], int c) {
     return to_f<T>(reinterpret_cast<const T*>(&raw[c >> 3])[c & 7]);
 }
 
+// The 8-bit operands' columns: w_scale[n0 + c] (c < kN) as raw 16-byte groups;
+// columns past n (a multiple of 8) read nothing and give zeros.
+template <int kN>
+__device__ __forceinline__ void fetch_scale(const float* w_scale, int n0, int n, float4 (&ws)[kN / 4]) {
+#pragma unroll
+    for (int q = 0; q < kN / 4; ++q)
+        ws[q] = n0 + 4 * q < n ? __ldg(reinterpret_cast<const float4*>(w_scale + n0) + q) : make_float4(0, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ void fetch_bias_n(const T* bias, int n0, int n, uint4 (&raw)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        raw[q] = bias != nullptr && n0 + 8 * q < n ? __ldg(reinterpret_cast<const uint4*>(bias + n0) + q)
+                                                   : make_uint4(0, 0, 0, 0);
+}
+// column d's scaled sum; both scales are multiplied first, as one token's and
+// one channel's scale
+template <int kN>
+__device__ __forceinline__ float scaled(uint32_t acc, const float4 (&ws)[kN / 4], int d, float as) {
+    const float4 w = ws[d >> 2];
+    const float s = (d & 3) == 0 ? w.x : ((d & 3) == 1 ? w.y : ((d & 3) == 2 ? w.z : w.w));
+    return static_cast<float>(static_cast<int32_t>(acc)) * (as * s);
+}
+
 // This lane's 128-byte row of its warp's staging box (16-byte chunk j at chunk
 // j ^ (row & 7): the tensor map's 128-byte swizzle, and no two lanes of a
 // quarter-warp on the same banks), written once the box's previous contents
@@ -148,13 +180,19 @@ __device__ __forceinline__ void stage_row(uint32_t srow, int lane, const uint32_
     __syncwarp();
 }
 
-template <typename T, int BN, int kEpi, bool kPair>
+// T: the operand type (of the bias and the 16-bit output, for 8-bit operands).
+template <typename T, int BN, int kEpi, bool kPair, bool kInt8 = false>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_cos,
                 const __grid_constant__ CUtensorMap map_sin, const Params p) {
     using S = Smem<BN, kPair, kEpi == kRope>;
     constexpr int kTileM = kPair ? 2 * kBM : kBM;
+    constexpr int kBKe = kInt8 ? kBK8 : kBK;
+    // epilogue warps with columns to write: a 64-column tile is one 64-column box per row group
+    constexpr int kActiveWarps = BN >= 128 ? kEpiWarps : kEpiWarps / 2;
+    constexpr int kWarpCols = BN >= 128 ? BN / 2 : BN;
+    static_assert(BN >= 128 || kInt8, "64-column tiles: 8-bit operands only");
     const uint32_t rank = kPair ? cluster_ctarank() : 0u;  // 0: the CTA that issues the MMAs
     const int unit0 = kPair ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
     const int units = kPair ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
@@ -168,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto bar = [&](int idx) { return sbase + S::bars + 8u * idx; };
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int kb_n = p.k / kBK;
+    const int kb_n = kInt8 ? (p.k + kBKe - 1) / kBKe : p.k / kBKe;  // 8-bit: the last stage zero-filled past k
 
     grid_launch_dependents();
     if (threadIdx.x == 0) {
@@ -178,11 +216,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bars[S::kAccFull + b], 1);
-            mbar_init(&bars[S::kAccEmpty + b], kPair ? 2 * kEpiWarps : kEpiWarps);  // one per epilogue warp
+            mbar_init(&bars[S::kAccEmpty + b], kPair ? 2 * kActiveWarps : kActiveWarps);  // one per epilogue warp
         }
         mbar_init(&bars[S::kDrain], 1);
         mbar_init(&bars[S::kCsFull], 1);
-        mbar_init(&bars[S::kCsEmpty], kEpiWarps);
+        mbar_init(&bars[S::kCsEmpty], kActiveWarps);
         st_shared_volatile_u32(ctl.misc + 4, 0);
         st_shared_u64(ctl.misc + 8, reinterpret_cast<uint64_t>(p.status));
         st_shared_u64(ctl.misc + 16, static_cast<uint64_t>(p.timeout_ns > 0 ? p.timeout_ns : kDefaultTimeoutNs));
@@ -236,12 +274,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // the even CTA's full barrier counts both CTAs' bytes; only it arms
                         const uint32_t fb = map_to_rank(bar(S::kFull + st), 0);
                         if (rank == 0) mbar_arrive_expect_tx(bar(S::kFull + st), 2 * (S::a_bytes + S::b_bytes));
-                        tma_load_2d_pair(sbase + S::a + st * S::a_bytes, &map_a, fb, kb * kBK, m0);
-                        tma_load_2d_pair(sbase + S::b + st * S::b_bytes, &map_b, fb, kb * kBK, n0);
+                        tma_load_2d_pair(sbase + S::a + st * S::a_bytes, &map_a, fb, kb * kBKe, m0);
+                        tma_load_2d_pair(sbase + S::b + st * S::b_bytes, &map_b, fb, kb * kBKe, n0);
                     } else {
                         mbar_arrive_expect_tx(bar(S::kFull + st), S::a_bytes + S::b_bytes);
-                        tma_load_2d(sbase + S::a + st * S::a_bytes, &map_a, bar(S::kFull + st), kb * kBK, m0);
-                        tma_load_2d(sbase + S::b + st * S::b_bytes, &map_b, bar(S::kFull + st), kb * kBK, n0);
+                        tma_load_2d(sbase + S::a + st * S::a_bytes, &map_a, bar(S::kFull + st), kb * kBKe, m0);
+                        tma_load_2d(sbase + S::b + st * S::b_bytes, &map_b, bar(S::kFull + st), kb * kBKe, n0);
                     }
                 }
                 __syncwarp();
@@ -260,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1 && rank == 0) {
         // ------------------------------------------------ MMA issuer
-        constexpr uint32_t idesc = idesc_f16(kTileM, BN, DTypeTraits<T>::kFormat, 0, 0);
+        constexpr uint32_t idesc = kInt8 ? idesc_s8(kTileM, BN) : idesc_f16(kTileM, BN, DTypeTraits<T>::kFormat, 0, 0);
         // completions go to both CTAs of a pair (their stages and accumulators)
         const auto commit = [&](int idx) {
             if constexpr (kPair) {
@@ -288,8 +326,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t da = sw128_desc(sbase + S::a + st * S::a_bytes);
                     const uint64_t db = sw128_desc(sbase + S::b + st * S::b_bytes);
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k) {
-                        if constexpr (kPair)
+                    for (int k = 0; k < kRowBytes / 32; ++k) {  // 32 bytes of K per instruction
+                        if constexpr (kPair && kInt8)
+                            mma_ss_i8_pair(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        else if constexpr (kInt8)
+                            mma_ss_i8(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        else if constexpr (kPair)
                             mma_ss_pair(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
                         else
                             mma_ss(tmem + buf * BN, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
@@ -343,10 +385,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             wait_bounded(bar(S::kCsFull), armed & 1, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
             __syncwarp();
         }
-    } else if (warp >= kEpiWarp0) {
+    } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kActiveWarps) {
         // ------------------------------------------------ epilogue
         const int wq = warp & 3;                       // TMEM lane quarter
-        const int c_begin = ((warp - kEpiWarp0) >> 2) * (BN / 2);  // this warp's column half
+        const int c_begin = ((warp - kEpiWarp0) >> 2) * kWarpCols;  // this warp's columns
         const int row = wq * 32 + lane;
         const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
         const uint32_t stg = sbase + S::stg + (warp - kEpiWarp0) * S::kStgBytes;
@@ -373,22 +415,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc_fence_after();
             const uint32_t tacc = tmem + lane_addr + buf * BN;
+            float as = 0.f;  // 8-bit operands: this row's scale
+            if constexpr (kInt8) as = m0 + row < p.m ? __ldg(p.a_scale + m0 + row) : 0.f;
             if constexpr (kEpi == kAccum) {
                 // fp32 boxes of 32 columns, added into the residual by TMA
 #pragma unroll 1
-                for (int q = 0; q < BN / 64; ++q) {
+                for (int q = 0; q < kWarpCols / 32; ++q) {
                     const int c = c_begin + 32 * q;
                     uint32_t acc[32];
                     uint4 braw[4];
+                    float4 ws[8];
                     tmem_ld32(tacc + c, acc);
-                    fetch_bias32<T>(bias, n0 + c, braw);
+                    if constexpr (kInt8) {
+                        fetch_bias_n<T>(bias, n0 + c, p.n, braw);
+                        fetch_scale<32>(p.w_scale, n0 + c, p.n, ws);
+                    } else {
+                        fetch_bias32<T>(bias, n0 + c, braw);
+                    }
                     tmem_wait_ld();
-                    if (q + 1 == BN / 64) acc_empty(buf);  // accumulator read out
+                    if (q + 1 == kWarpCols / 32) acc_empty(buf);  // accumulator read out
                     uint32_t w[32];
 #pragma unroll
-                    for (int d = 0; d < 32; ++d) w[d] = __float_as_uint(__uint_as_float(acc[d]) + bias_at<T>(braw, d));
+                    for (int d = 0; d < 32; ++d)
+                        w[d] = __float_as_uint((kInt8 ? scaled<32>(acc[d], ws, d, as) : __uint_as_float(acc[d])) +
+                                               bias_at<T>(braw, d));
                     stage_row(srow, lane, w);
-                    if (lane == 0 && live) {
+                    if (lane == 0 && live && (!kInt8 || n0 + c < p.n)) {
                         tma_reduce_add_2d(&map_out, stg, n0 + c, y0);
                         bulk_commit_group();
                     }
@@ -430,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 warp_arrive(bar(S::kCsEmpty), lane);  // the rows are in registers
                 const int sw = lane & 7;
 #pragma unroll 1
-                for (int c = c_begin; c < c_begin + BN / 2; c += 64) {
+                for (int c = c_begin; c < c_begin + kWarpCols; c += 64) {
                     const bool rot = n0 + c < p.rope_cols;
                     if (lane == 0) bulk_wait_read_all();  // the box's previous head has been copied out
                     __syncwarp();
@@ -438,18 +490,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int d0 = 0; d0 < 32; d0 += 16) {  // pairs (d, d + 32), 16 at a time
                         uint32_t lo[16], hi[16];
                         uint4 bl[2], bh[2];
+                        float4 wl[4], wh[4];
+                        const bool in_n = !kInt8 || n0 + c < p.n;  // whole heads: n is a multiple of 64
                         tmem_ld16(tacc + c + d0, lo);
                         tmem_ld16(tacc + c + 32 + d0, hi);
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            bl[q] = bias != nullptr ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + d0) + q)
+                            bl[q] = bias != nullptr && in_n ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + d0) + q)
                                                     : make_uint4(0, 0, 0, 0);
-                            bh[q] = bias != nullptr
+                            bh[q] = bias != nullptr && in_n
                                         ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + 32 + d0) + q)
                                         : make_uint4(0, 0, 0, 0);
                         }
+                        if constexpr (kInt8) {
+                            fetch_scale<16>(p.w_scale, n0 + c + d0, p.n, wl);
+                            fetch_scale<16>(p.w_scale, n0 + c + 32 + d0, p.n, wh);
+                        }
                         tmem_wait_ld();
                         float a[16], b[16];
+                        if constexpr (kInt8) {  // rounded once, after the rotation
+#pragma unroll
+                            for (int d = 0; d < 16; ++d) {
+                                a[d] = scaled<16>(lo[d], wl, d, as) + to_f<T>(reinterpret_cast<const T*>(bl)[d]);
+                                b[d] = scaled<16>(hi[d], wh, d, as) + to_f<T>(reinterpret_cast<const T*>(bh)[d]);
+                            }
+                        } else
 #pragma unroll
                         for (int d = 0; d < 16; ++d) {
                             a[d] = round_t<T>(__uint_as_float(lo[d]) + to_f<T>(reinterpret_cast<const T*>(bl)[d]));
@@ -479,10 +544,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
-                    if (c + 64 == c_begin + BN / 2) acc_empty(buf);
+                    if (c + 64 == c_begin + kWarpCols) acc_empty(buf);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0 && live) {
+                    if (lane == 0 && live && (!kInt8 || n0 + c < p.n)) {
                         tma_store_2d(&map_out, stg, n0 + c, y0);
                         bulk_commit_group();
                     }
@@ -490,16 +555,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
                 // kStore: 64-column boxes
 #pragma unroll 1
-                for (int c = c_begin; c < c_begin + BN / 2; c += 64) {
+                for (int c = c_begin; c < c_begin + kWarpCols; c += 64) {
                     uint32_t a0[32], a1[32];
                     uint4 b0[4], b1[4];
                     tmem_ld32(tacc + c, a0);
                     tmem_ld32(tacc + c + 32, a1);
-                    fetch_bias32<T>(bias, n0 + c, b0);
-                    fetch_bias32<T>(bias, n0 + c + 32, b1);
+                    if constexpr (kInt8) {
+                        fetch_bias_n<T>(bias, n0 + c, p.n, b0);
+                        fetch_bias_n<T>(bias, n0 + c + 32, p.n, b1);
+                    } else {
+                        fetch_bias32<T>(bias, n0 + c, b0);
+                        fetch_bias32<T>(bias, n0 + c + 32, b1);
+                    }
                     tmem_wait_ld();
-                    if (c + 64 == c_begin + BN / 2) acc_empty(buf);
+                    if (c + 64 == c_begin + kWarpCols) acc_empty(buf);
                     uint32_t w[32];
+                    if constexpr (kInt8) {
+                        float4 ws[8];
+                        fetch_scale<32>(p.w_scale, n0 + c, p.n, ws);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q)
+                            w[q] = DTypeTraits<T>::pack(scaled<32>(a0[2 * q], ws, 2 * q, as) + bias_at<T>(b0, 2 * q),
+                                                        scaled<32>(a0[2 * q + 1], ws, 2 * q + 1, as) +
+                                                            bias_at<T>(b0, 2 * q + 1));
+                        fetch_scale<32>(p.w_scale, n0 + c + 32, p.n, ws);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q)
+                            w[16 + q] = DTypeTraits<T>::pack(
+                                scaled<32>(a1[2 * q], ws, 2 * q, as) + bias_at<T>(b1, 2 * q),
+                                scaled<32>(a1[2 * q + 1], ws, 2 * q + 1, as) + bias_at<T>(b1, 2 * q + 1));
+                    } else
 #pragma unroll
                     for (int q = 0; q < 16; ++q) {
                         w[q] = DTypeTraits<T>::pack(__uint_as_float(a0[2 * q]) + bias_at<T>(b0, 2 * q),
@@ -508,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                          __uint_as_float(a1[2 * q + 1]) + bias_at<T>(b1, 2 * q + 1));
                     }
                     stage_row(srow, lane, w);
-                    if (lane == 0 && live) {
+                    if (lane == 0 && live && (!kInt8 || n0 + c < p.n)) {
                         tma_store_2d(&map_out, stg, n0 + c, y0);
                         bulk_commit_group();
                     }

@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define FDS_ABI_VERSION 4
+#define FDS_ABI_VERSION 5
 
 #if defined(_WIN32)
 #define FDS_API __declspec(dllexport)
@@ -270,6 +270,141 @@ typedef struct FdsLinearArgs {
 } FdsLinearArgs;
 
 FDS_API int fds_linear_fwd(const FdsLinearArgs* args, void* stream);
+
+/*
+ * The linear layer over 8-bit integers: out[m, n] from
+ *   D[m, n] = (sum_k a[m, k] w[n, k]) * (a_scale[m] * w_scale[n])
+ * with the epilogues of fds_linear_fwd (FDS_EPILOGUE_ROPE rotates D + bias in
+ * fp32 and rounds once). a holds one fp32 scale per row (token), w one per row
+ * (output channel); the products are summed exactly in 32-bit integers. Up to
+ * 8 rows of a run on a kernel that reads w once over all SMs, more on the
+ * tensor cores. k must be a multiple of 16 and at most 65536, n a multiple of 8
+ * (of 64 for FDS_EPILOGUE_ROPE); m = 0 is a no-op. No counterpart in the
+ * reference (its projections are fp16: triton/src/fds_triton/model.py:50-57).
+ */
+typedef struct FdsLinearInt8Args {
+    const void* a;            /* device int8 [m, a_row_stride] */
+    int64_t a_row_stride;     /* elements; multiple of 16, >= k */
+    const float* a_scale;     /* device fp32 [m] */
+    const void* w;            /* device int8 [n, w_row_stride] */
+    int64_t w_row_stride;     /* elements; multiple of 16, >= k */
+    const float* w_scale;     /* device fp32 [n], 16-byte aligned */
+    const void* bias;         /* device, dtype, [n], or NULL */
+    void* out;                /* device, [m, out_row_stride]: dtype, or fp32 for ACCUMULATE_F32 */
+    int64_t out_row_stride;   /* elements; multiple of 8 (4 for fp32), >= n */
+    const float* cos;         /* FDS_EPILOGUE_ROPE only: fp32 [>= seq_len, 64] */
+    const float* sin;
+    int32_t* status;          /* device word for bounded-wait errors, or NULL */
+    int32_t* status_host;     /* mapped pinned host mirror, or NULL */
+    int32_t m;
+    int32_t n;
+    int32_t k;
+    int32_t dtype;            /* FDS_DTYPE_* of bias and out (unless ACCUMULATE_F32) */
+    int32_t epilogue;         /* FDS_EPILOGUE_* */
+    int32_t seq_len;          /* FDS_EPILOGUE_ROPE: position = row % seq_len */
+    int32_t rope_cols;        /* FDS_EPILOGUE_ROPE: multiple of 64, <= n */
+    int64_t timeout_ns;       /* bound on every in-kernel wait; <= 0 selects 2 s */
+    int32_t tile_n;           /* 0 = by shape; 64, 128 or 256 columns per tensor-core tile */
+    int32_t cta_pair;         /* FDS_GEMM_* */
+} FdsLinearInt8Args;
+
+FDS_API int fds_linear_int8_fwd(const FdsLinearInt8Args* args, void* stream);
+
+/*
+ * The step between two blocks, over rows of c elements:
+ *   z = post(y) * post_w + post_b
+ *   x_out = alpha * x + gate * z
+ *   h = (norm(x_out) * w + b) * (1 + scale) + shift
+ * Without y (NULL) x_out is x. h uses the 32-bit x_out, before its rounding to
+ * the stream's type. With h_scale h is int8, quantised per row: h_scale = max|h| / 127,
+ * q = rint(h * (127 / max|h|)) (ties to even), so FDS_NORM_NONE without y is the
+ * row quantiser of fds_linear_int8_fwd; a row whose maximum is below 2^-100 is
+ * zero with scale 0, one with an infinity or a NaN gets the scale NaN. Every
+ * vector may be NULL (absent). gate, scale and shift are [c], or one row per
+ * window (gate_stride / mod_stride > 0): row r reads window r / length. x_out may
+ * be x. c must be a multiple of 8, at most 16384.
+ * Replaces: triton/src/fds_triton/kernels.py:61 _res_norm_kernel (residual add,
+ * LayerNorm, adaLN modulation), with the norm after the block added.
+ */
+#define FDS_NORM_NONE 0
+#define FDS_NORM_LAYER 1
+#define FDS_NORM_RMS 2
+
+typedef struct FdsResidualNormArgs {
+    const void* x;            /* device, fp32 (x_f32) or dtype, [rows, x_stride] */
+    int64_t x_stride;         /* elements; rows 16-byte aligned, likewise below */
+    const void* y;            /* device, dtype, [rows, y_stride], or NULL */
+    int64_t y_stride;
+    void* x_out;              /* device, x's type; or NULL without y */
+    int64_t x_out_stride;
+    void* h;                  /* device, dtype (int8 with h_scale), or NULL */
+    int64_t h_stride;
+    float* h_scale;           /* device fp32 [rows], or NULL */
+    const void* gate;         /* parameter vectors: fp32 (param_f32) or dtype */
+    int64_t gate_stride;
+    const void* post_w;
+    const void* post_b;
+    const void* w;
+    const void* b;
+    const void* scale;
+    const void* shift;
+    int64_t mod_stride;
+    int32_t rows;
+    int32_t c;
+    int32_t length;           /* rows per window */
+    int32_t dtype;            /* FDS_DTYPE_* */
+    int32_t x_f32;
+    int32_t param_f32;
+    int32_t post;             /* FDS_NORM_* after the block (over y) */
+    int32_t norm;             /* FDS_NORM_* before the next block (over x_out) */
+    float alpha;
+    float eps;
+} FdsResidualNormArgs;
+
+FDS_API int fds_residual_norm_fwd(const FdsResidualNormArgs* args, void* stream);
+
+/*
+ * Attention over a sliding window of keys and a few first keys that stay
+ * visible (sinks). Query i of window b sits at position p = q_start[b] + i of
+ * the keys and sees key j iff j < kv_len[b], j <= p + right and (j >= p - left
+ * or j < sinks); out = softmax over the keys it sees, times V, and 0 for a query
+ * that sees none. q / out [batch, q_len, heads, 64], k / v [batch, k_len,
+ * kv_heads, 64] with any strides (batch, row, head; multiples of 8 elements);
+ * query head h reads key head h / (heads / kv_heads). Keys and values that no
+ * query of its 128-row tile sees (unwritten cache rows, rows past kv_len) may hold anything,
+ * infinities and NaN included. Up to 8 query rows per key head (q_len * heads /
+ * kv_heads) run on a kernel without tensor cores, split over the keys.
+ * No counterpart in the reference, whose windows end at 120 s
+ * (triton/src/fds_triton/runtime.py:179).
+ */
+typedef struct FdsWindowArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    int64_t q_stride[3];      /* elements: batch, row, head */
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t out_stride[3];
+    const int32_t* q_start;   /* device [batch], or NULL (0) */
+    const int32_t* kv_len;    /* device [batch], or NULL (k_len) */
+    int32_t* status;          /* device word for bounded-wait errors, or NULL */
+    int32_t* status_host;     /* mapped pinned host mirror, or NULL */
+    int32_t batch;
+    int32_t heads;
+    int32_t kv_heads;
+    int32_t q_len;
+    int32_t k_len;
+    int32_t head_dim;         /* must be 64 */
+    int32_t dtype;            /* FDS_DTYPE_* */
+    int32_t left;
+    int32_t right;
+    int32_t sinks;
+    float scale;              /* softmax scale on q . k */
+    int64_t timeout_ns;       /* bound on every in-kernel wait; <= 0 selects 2 s */
+} FdsWindowArgs;
+
+FDS_API int fds_window_attn_fwd(const FdsWindowArgs* args, void* stream);
 
 /* Version of this ABI (FDS_ABI_VERSION). */
 FDS_API int fds_abi_version(void);

@@ -1,0 +1,413 @@
+"""Window attention with sinks, the 8-bit projections and the residual norm
+against their 64-bit definitions (oracle/layer_oracle.py).
+
+Tolerances, with u the unit roundoff of the 16-bit type (2^-11 fp16, 2^-8 bf16)
+and v = 2^-24 that of fp32:
+
+* window attention: the weights are rounded to the operand type for the P V
+  product and the output once more, each at most u max|v| away; the
+  exponentials are within 7.5e-5 relative (the polynomial), which a normalised
+  sum at most doubles: (2 u + 2e-4) max|v|.
+* 8-bit projections: the integer sum is exact; three fp32 roundings of the
+  product, one of the bias sum (the rotation adds three), then u of the result:
+  u |y| + 8 v (|product| + |b|), with the fp16 subnormal half step 2^-25. The
+  fp32 accumulate form: 8 v (|product| + |b| + |x|).
+* residual norm: a row's sums pass at most 72 roundings (64 per thread, 8 levels
+  across threads), applied to two norms: 2^-17 of the row's largest term, plus u
+  |h| for a 16-bit h and u |x'| for a 16-bit stream.
+* row quantisation: equal, value for value (its definition is in fp32).
+"""
+
+import pytest
+import torch
+
+import fastdialoguesidon_b200 as F
+from oracle import layer_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+V = 2.0 ** -24
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---------------------------------------------------------------- window attention
+
+
+def _check_window(q, k, v, left, right=0, sinks=0, q_start=None, kv_len=None, out=None, clean_v=None):
+    ref = O.window_attention(q.cpu(), k.cpu(), v.cpu(), left, right, sinks,
+                             None if q_start is None else q_start.cpu(), None if kv_len is None else kv_len.cpu())
+    got = F.window_attention(q, k, v, left, right, sinks, q_start=q_start, kv_len=kv_len, out=out)
+    F.check_status()
+    if out is not None:
+        assert got.data_ptr() == out.data_ptr()
+    vmax = float((v if clean_v is None else clean_v).float().abs().max())
+    bound = (2 * U[q.dtype] + 2e-4) * vmax
+    err = float((got.cpu().double() - ref).abs().max())
+    assert err <= bound, (err, bound)
+    return got, ref
+
+
+def _qkv(B, Lq, Lk, H, Hk, dtype, seed):
+    g = _gen(seed)
+    return tuple(torch.randn(B, n, h, 64, generator=g).to(dtype).cuda() for n, h in ((Lq, H), (Lk, Hk), (Lk, Hk)))
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("L,left,right,sinks", [
+    (1, 5, 0, 0), (9, 3, 2, 1), (127, 40, 0, 4), (128, 128, 128, 0), (129, 1, 0, 7), (300, 64, 64, 8), (517, 100, 30, 16),
+    (640, 255, 0, 130), (333, 10000, 10000, 3), (400, 0, 0, 0), (700, 37, 5, 300)])
+def test_window_self_attention(cuda_device, dtype, L, left, right, sinks):
+    """Sizes around the tile: windows shorter and longer than a tile, windows past
+    both ends, sinks inside a tile, at its edge, over several tiles."""
+    q, k, v = _qkv(2, L, L, 2, 2, dtype, seed=L + left)
+    _check_window(q, k, v, left, right, sinks)
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk", [(1, 1, 1000, 12, 12), (3, 1, 777, 8, 2), (2, 1, 64, 8, 1), (2, 2, 500, 4, 4),
+                                          (1, 3, 900, 4, 2), (2, 7, 333, 3, 3), (1, 5, 257, 2, 2), (1, 8, 4100, 1, 1)])
+@pytest.mark.parametrize("left,right,sinks", [(50, 0, 0), (400, 0, 4), (90, 3, 70), (100000, 0, 1)])
+def test_window_steps(cuda_device, B, Lq, Lk, H, Hk, left, right, sinks):
+    """Up to 8 query rows per key head, every row count, shared key heads."""
+    q, k, v = _qkv(B, Lq, Lk, H, Hk, torch.float16, seed=Lk + left)
+    start = torch.tensor([max(0, Lk - Lq - 40 * b) for b in range(B)], dtype=torch.int32, device="cuda")
+    _check_window(q, k, v, left, right, sinks, q_start=start)
+
+
+@pytest.mark.parametrize("Lq,left,sinks", [(9, 3000, 4), (40, 2000, 0), (128, 5000, 16), (130, 1500, 200)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_window_chunk_split_over_a_cluster(cuda_device, dtype, Lq, left, sinks):
+    """Few query tiles, many key tiles: a unit's tiles dealt to up to 8 CTAs and merged."""
+    q, k, v = _qkv(1, Lq, 4133, 2, 1, dtype, seed=Lq)
+    _check_window(q, k, v, left, 0, sinks, q_start=_i32(4133 - Lq))
+
+
+def test_window_shared_key_heads_in_tiles(cuda_device):
+    q, k, v = _qkv(2, 200, 320, 6, 2, torch.float16, seed=3)
+    _check_window(q, k, v, 70, 10, 5, q_start=_i32(0, 100))
+
+
+@pytest.mark.parametrize("Lq", [1, 3, 150])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_window_unseen_rows_may_hold_anything(cuda_device, Lq, bad):
+    """A cache's unwritten tail and rows past kv_len, in K and in V; and, for
+    single steps, everything between the sinks and the window."""
+    q, k, v = _qkv(2, Lq, 900, 2, 2, torch.float16, seed=Lq)
+    kb, vb = k.clone(), v.clone()
+    start = _i32(500, 333)
+    for b, s in enumerate((500, 333)):
+        kb[b, s + Lq:], vb[b, s + Lq:] = bad, bad
+        lo = s - 60
+        if Lq == 1:
+            kb[b, 4:lo], vb[b, 4:lo] = bad, bad
+    got, _ = _check_window(q, kb, vb, 60, 0, 4, q_start=start, clean_v=v)
+    assert torch.isfinite(got).all()
+    # the same through kv_len with keys to the right of the window allowed
+    kb, vb = k.clone(), v.clone()
+    for b, n in enumerate((470, 900)):
+        kb[b, n:], vb[b, n:] = bad, bad
+    got, _ = _check_window(q, kb, vb, 60, 100, 4, q_start=start, kv_len=_i32(470, 900), clean_v=v)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("Lq", [1, 2, 130])
+def test_window_rows_that_see_nothing(cuda_device, Lq):
+    """kv_len 0; a window wholly past kv_len; positions before the first key."""
+    q, k, v = _qkv(3, Lq, 400, 2, 2, torch.float16, seed=7)
+    v[0, 0] = float("inf")
+    got, ref = _check_window(q, k, v, 20, 0, 0, q_start=_i32(100, 390, -1000), kv_len=_i32(0, 300, 400),
+                             clean_v=torch.randn(4, device="cuda"))
+    assert float(ref.abs().max()) == 0.0 and float(got.abs().max()) == 0.0
+    got, ref = _check_window(q, k, v, 20, 0, 3, q_start=_i32(100, 390, -1000), kv_len=_i32(0, 300, 400))
+    assert float(got[0].abs().max()) == 0.0 and float(got[2].abs().max()) == 0.0  # the sinks lie ahead of window 2
+    assert float(got[1].abs().max()) > 0.0
+
+
+def test_window_views_and_out(cuda_device):
+    """q, k, v as column blocks of a qkv projection; a [B, H, L, 64] cache; a strided out."""
+    g = _gen(11)
+    B, L, H = 2, 203, 3
+    qkv = torch.randn(B * L, 3 * H * 64 + 64, generator=g).half().cuda()[:, :3 * H * 64]
+    s = qkv.stride(0)
+    q, k, v = (torch.as_strided(qkv, (B, L, H, 64), (L * s, s, 64, 1), i * H * 64) for i in range(3))
+    wide = torch.zeros(B, L, H, 128, dtype=torch.float16, device="cuda")
+    _check_window(q, k, v, 33, 12, 2, out=wide[..., :64])
+    assert float(wide[..., 64:].abs().max()) == 0.0
+    cache_k, cache_v = (torch.randn(B, H, 500, 64, generator=g).half().cuda().transpose(1, 2) for _ in range(2))
+    for n in (1, 5, 60):
+        _check_window(q[:, :n], cache_k, cache_v, 90, 0, 2, q_start=_i32(300, 450 - n))
+
+
+def test_window_matches_full_attention_when_wide(cuda_device):
+    """A window over everything is the bidirectional attention of rotated_attention."""
+    g = _gen(5)
+    B, L, H = 2, 500, 4
+    qkv = torch.randn(B * L, 3 * H * 64, generator=g).half().cuda()
+    t = qkv.view(B, L, 3, H, 64)
+    a = F.window_attention(t[:, :, 0], t[:, :, 1], t[:, :, 2], L, L).reshape(B * L, H * 64)
+    b = F.rotated_attention(qkv, B, H)
+    assert float((a.float() - b.float()).abs().max()) <= 2 * (2 * U[torch.float16] + 2e-4) * float(qkv.abs().max())
+
+
+def test_window_empty_and_repeat(cuda_device):
+    q, k, v = _qkv(1, 300, 300, 2, 2, torch.float16, seed=2)
+    assert F.window_attention(q[:, :0], k, v, 5).shape == (1, 0, 2, 64)
+    assert float(F.window_attention(q, k[:, :0], v[:, :0], 5).abs().max()) == 0.0
+    a = F.window_attention(q[:, :20], k, v, 200, 0, 4, q_start=_i32(250))
+    for _ in range(5):
+        assert torch.equal(a, F.window_attention(q[:, :20], k, v, 200, 0, 4, q_start=_i32(250)))
+
+
+# ---------------------------------------------------------------- 8-bit projections
+
+
+def _int8_operands(m, k, n, dtype, bias, seed):
+    g = _gen(seed)
+    x = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+    xs = torch.rand(m, generator=g) * 1e-3 + 1e-4
+    ws = torch.rand(n, generator=g) * 1e-3 + 1e-4
+    b = (torch.randn(n, generator=g) * 0.1).to(dtype) if bias else None
+    return x, xs, w, ws, b
+
+
+def _cuda(*ts):
+    return tuple(None if t is None else t.cuda() for t in ts)
+
+
+def _check_linear(got, prod, ref, dtype, extra=0.0):
+    bound = U[dtype] * ref.abs() + 8 * V * (prod.abs() + (ref - prod).abs() + extra) + 2.0 ** -25
+    err = (got.cpu().double() - ref).abs()
+    assert bool((err <= bound).all()), float((err - bound).max())
+
+
+SHAPES = [(1, 16, 8), (1, 768, 2304), (2, 1024, 1024), (3, 144, 200), (5, 4096, 72), (8, 1040, 264), (9, 16, 8), (33, 112, 136),
+          (128, 128, 64), (129, 256, 328), (200, 1024, 1000), (257, 2064, 512), (1000, 768, 2304), (700, 1024, 4104)]
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_linear_int8(cuda_device, m, k, n, dtype):
+    x, xs, w, ws, b = _int8_operands(m, k, n, dtype, bias=m % 2 == 1, seed=m + n)
+    prod, ref = O.linear_int8(x, xs, w, ws, b)
+    got = F.linear_int8(*_cuda(x, xs, w, ws, b), dtype=dtype)
+    F.check_status()
+    assert got.dtype == dtype
+    _check_linear(got, prod, ref, dtype)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 768, 264), (8, 256, 72), (40, 144, 328), (300, 1024, 520), (700, 400, 1024)])
+def test_accumulate_int8(cuda_device, m, k, n):
+    x, xs, w, ws, b = _int8_operands(m, k, n, torch.float16, bias=True, seed=m)
+    r = torch.randn(m, n + 4 if n % 16 else n, generator=_gen(m)).cuda()[:, :n]
+    r0 = r.cpu().double()
+    prod, ref = O.linear_int8(x, xs, w, ws, b)
+    F.accumulate_int8(r, *_cuda(x, xs, w, ws, b))
+    F.check_status()
+    err = (r.cpu().double() - (r0 + ref)).abs()
+    assert bool((err <= 8 * V * (prod.abs() + b.double().abs() + r0.abs())).all())
+
+
+@pytest.mark.parametrize("m,length,heads", [(1, 6000, 12), (7, 3, 2), (50, 50, 3), (333, 111, 2), (600, 600, 12), (260, 6000, 1)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_linear_int8_rope(cuda_device, m, length, heads, dtype):
+    n = 3 * heads * 64
+    x, xs, w, ws, b = _int8_operands(m, 144, n, dtype, bias=True, seed=m)
+    cos, sin = F.rope_tables(min(length, m))
+    prod, ref = O.linear_int8(x, xs, w, ws, b)
+    mag = prod.abs() + b.double().abs()
+    pair = mag.clone()
+    for at in range(0, 2 * heads * 64, 64):
+        pair[:, at:at + 64] += torch.cat([mag[:, at + 32:at + 64], mag[:, at:at + 32]], 1)
+    ref = O.rope(ref, cos, sin, length, 2 * heads * 64)
+    xd, xsd, wd, wsd, bd = _cuda(x, xs, w, ws, b)
+    got = F.linear_int8_rope(xd, xsd, wd, wsd, bd, cos.cuda(), sin.cuda(), length, heads, dtype=dtype)
+    F.check_status()
+    bound = U[dtype] * ref.abs() + 8 * V * pair + 2.0 ** -25
+    assert bool(((got.cpu().double() - ref).abs() <= bound).all())
+
+
+def test_int8_tilings_agree_bit_for_bit(cuda_device):
+    """Every tensor-core tiling, and the few-rows kernel against them."""
+    for m, k, n in ((5, 768, 520), (300, 1040, 776)):
+        ops = _cuda(*_int8_operands(m, k, n, torch.float16, bias=True, seed=1))
+        ref = F.linear_int8(*ops)
+        for pair, tile_n in ((False, 64), (False, 128), (False, 256), (True, 128), (True, 256)):
+            assert torch.equal(ref, F.linear_int8(*ops, pair=pair, tile_n=tile_n)), (m, pair, tile_n)
+    F.check_status()
+
+
+def test_int8_extreme_values_and_strides(cuda_device):
+    """-128 and 127 throughout (the largest sums), column slices of wider buffers, out=."""
+    m, k, n = 70, 2048, 136
+    x = torch.full((m, k + 32), -128, dtype=torch.int8, device="cuda")[:, 16:16 + k]
+    w = torch.full((n, k + 16), -128, dtype=torch.int8, device="cuda")[:, :k]
+    w[1::2] = 127
+    one = torch.full((m,), 2.0 ** -12, device="cuda")
+    ws = torch.full((n,), 2.0 ** -8, device="cuda")
+    out = torch.full((m, n + 8), 7.0, dtype=torch.float16, device="cuda")
+    for rows in (3, m):
+        got = F.linear_int8(x[:rows], one[:rows], w, ws, out=out[:rows, :n])
+        prod, ref = O.linear_int8(x[:rows].cpu(), one[:rows].cpu(), w.cpu(), ws.cpu())
+        _check_linear(got, prod, ref, torch.float16)
+    assert float(out[:, n:].min()) == 7.0
+
+
+@pytest.mark.parametrize("rows,c", [(1, 8), (5, 64), (33, 768), (100, 1024), (7, 1160), (9, 2048), (4, 4096), (3, 5000), (2, 16384)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_quantize_rows(cuda_device, rows, c, dtype):
+    g = _gen(rows + c)
+    x = (torch.randn(rows, c, generator=g) * torch.exp(2 * torch.randn(rows, 1, generator=g))).to(dtype)
+    if rows > 3:
+        x[1] = 0
+        x[2] = 0
+        x[2, 3] = -1.0
+    q, s = F.quantize_rows(x.cuda())
+    qr, sr = O.quantize_rows(x)
+    assert torch.equal(q.cpu(), qr) and torch.equal(s.cpu(), sr)
+
+
+def test_quantize_rows_not_finite(cuda_device):
+    x = torch.ones(4, 64, dtype=torch.float16)
+    x[0, 5], x[1, 6], x[2, 7] = float("nan"), float("inf"), -float("inf")
+    q, s = F.quantize_rows(x.cuda())
+    assert torch.isnan(s[:3]).all() and float(s[3]) == float(torch.tensor(1.0) / 127)
+    assert F.quantize_rows(x[:0].cuda())[0].shape == (0, 64)
+
+
+# ---------------------------------------------------------------- residual norm
+
+
+def _norm_case(rows, c, dtype, stream, post, norm, gate, mod, windows, pdtype, seed):
+    g = _gen(seed)
+
+    def rnd(*shape, scale=1.0, dt=pdtype):
+        return (torch.randn(*shape, generator=g) * scale).to(dt)
+
+    return dict(
+        x=rnd(rows, c, scale=3.0, dt=stream), y=rnd(rows, c, scale=2.0, dt=dtype),
+        gate={"none": None, "layer": rnd(c), "window": rnd(windows, c)}[gate],
+        post=post, post_weight=None if post == "none" else rnd(c), post_bias=rnd(c) if post == "layer" else None,
+        norm=norm, weight=rnd(c), bias=rnd(c) if norm == "layer" else None,
+        scale=rnd(windows, c) if mod else None, shift=rnd(windows, c) if mod else None, length=-(-rows // windows))
+
+
+def _to(d):
+    return {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+
+
+def _terms(case, x, h):
+    """The largest term of each row of x' and of h, for the bounds."""
+    _, hx = O.residual_norm(**{**case, "shift": None, "bias": None})
+    z = O._norm(case["y"].double(), case["post"], case["post_weight"], None, 1e-5) if case["y"] is not None else x * 0
+    big_x = (case["x"].double().abs() + (z.abs() + 1) * (1 if case["gate"] is None else 1 + case["gate"].double().abs().max())).amax(1, keepdim=True)
+    mod = 1 if case["scale"] is None else 1 + case["scale"].double().abs().max()
+    return big_x, (hx.abs() + h.abs()).amax(1, keepdim=True) * mod + mod * (0 if case["bias"] is None else case["bias"].double().abs().max())
+
+
+NORMS = [
+    (1, 768, "none", "layer", "window", True, 1), (33, 8, "none", "layer", "none", False, 1), (100, 768, "rms", "rms", "layer", False, 3),
+    (77, 1024, "layer", "layer", "window", True, 4), (50, 1160, "rms", "layer", "window", True, 2), (19, 2048, "layer", "rms", "layer", True, 1),
+    (9, 4096, "none", "none", "layer", False, 1), (5, 8192, "layer", "layer", "none", True, 5), (3, 16384, "rms", "rms", "window", True, 2)]
+
+
+@pytest.mark.parametrize("rows,c,post,norm,gate,mod,windows", NORMS)
+@pytest.mark.parametrize("dtype,stream,pdtype", [(torch.float16, torch.float32, torch.float16), (torch.bfloat16, torch.bfloat16, torch.bfloat16),
+                                                 (torch.bfloat16, torch.float32, torch.float32), (torch.float16, torch.float16, torch.float32)])
+def test_residual_norm(cuda_device, rows, c, post, norm, gate, mod, windows, dtype, stream, pdtype):
+    case = _norm_case(rows, c, dtype, stream, post, norm, gate, mod, windows, pdtype, seed=rows + c)
+    rx, rh = O.residual_norm(residual_scale=0.5, **case)
+    big_x, big_h = _terms(case, rx, rh)
+    dev = _to(case)
+    x0 = dev["x"].clone()
+    keep = torch.empty_like(x0)
+    x1, h = F.residual_norm(residual_scale=0.5, residual_out=keep, **dev)
+    assert x1.data_ptr() == keep.data_ptr() and torch.equal(dev["x"], x0)
+    ux = 0.0 if stream == torch.float32 else U[stream]
+    assert bool(((x1.cpu().double() - rx).abs() <= ux * rx.abs() + 2.0 ** -17 * big_x).all())
+    assert h.dtype == dtype
+    assert bool(((h.cpu().double() - rh).abs() <= U[dtype] * rh.abs() + 2.0 ** -17 * big_h + 2.0 ** -25).all())
+    # quantised rows of the same h: each value within half a step of it
+    _, (q, s) = F.residual_norm(residual_scale=0.5, residual_out=keep, quantize=True, **dev)
+    s = s.cpu().double()[:, None]
+    assert bool(((s - rh.abs().amax(1, keepdim=True) / 127).abs() <= 2.0 ** -17 * big_h / 127 + 4 * V * s).all())
+    assert bool(((q.cpu().double() * s - rh).abs() <= s / 2 + 2.0 ** -17 * big_h * 2 + 4 * V * 127 * s).all())
+    # in place
+    x2, h2 = F.residual_norm(residual_scale=0.5, **dev)
+    assert x2.data_ptr() == dev["x"].data_ptr() and torch.equal(x2, x1) and torch.equal(h2, h)
+
+
+def test_residual_norm_without_a_block(cuda_device):
+    case = _norm_case(41, 768, torch.float16, torch.float32, "none", "layer", "none", True, 2, torch.float16, seed=1)
+    case["y"] = None
+    rx, rh = O.residual_norm(**case)
+    _, big = _terms(case, rx, rh)
+    dev = _to(case)
+    x, h = F.residual_norm(**dev)
+    assert x.data_ptr() == dev["x"].data_ptr() and torch.equal(x.cpu(), case["x"])
+    assert bool(((h.cpu().double() - rh).abs() <= U[torch.float16] * rh.abs() + 2.0 ** -17 * big + 2.0 ** -25).all())
+
+
+def test_residual_norm_strided_rows_and_constant_rows(cuda_device):
+    """Column slices; a row without variance (the root holds eps alone); a row far from zero."""
+    g = _gen(9)
+    wide = torch.randn(30, 512, generator=g).cuda()
+    wide[3, 64:320] = 5.0
+    wide[4, 64:320] += 3000.0
+    y = torch.zeros(30, 264, dtype=torch.float16, device="cuda")[:, 8:]
+    out = torch.zeros(30, 320, dtype=torch.float16, device="cuda")
+    x = wide[:, 64:320]
+    rx, rh = O.residual_norm(x.cpu(), y.cpu())
+    x1, h = F.residual_norm(x, y, out=out[:, :256])
+    assert torch.equal(x1.cpu().double(), rx)
+    assert float(h[3].abs().max()) == 0.0
+    # |x| / deviation is 3000 in row 4: the mean's rounding counts that much more
+    tol = torch.full((30, 1), 2.0 ** -17).double()
+    tol[4] *= 3000
+    assert bool(((h.cpu().double() - rh).abs() <= U[torch.float16] * rh.abs() + tol * rh.abs().amax(1, keepdim=True)).all())
+    assert float(out[:, 256:].abs().max()) == 0.0
+
+
+# ---------------------------------------------------------------- together
+
+
+def test_on_another_stream_and_in_a_graph(cuda_device):
+    """The ops follow the current stream, and replay from a CUDA graph."""
+    L, C, H = 260, 768, 12
+    x, xs, w, ws, b = _cuda(*_int8_operands(L, C, 3 * C, torch.float16, bias=True, seed=4))
+    ws = ws * 0.05
+    cos, sin = F.rope_tables(L, "cuda")
+    y = torch.randn(L, C, generator=_gen(2)).half().cuda()
+    r = torch.randn(L, C, generator=_gen(3)).cuda()
+    keep = torch.empty_like(r)
+
+    def layer():
+        qkv = F.linear_int8_rope(x, xs, w, ws, b, cos, sin, L, H).view(1, L, 3, H, 64)
+        ctx = F.window_attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], 64, 64, 4).view(L, C)
+        _, (hq, hs) = F.residual_norm(r, ctx + y, residual_out=keep, quantize=True)
+        return ctx, F.linear_int8(hq, hs, w, ws, b)
+
+    want = layer()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = layer()
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = layer()
+    for t in held:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    F.check_status()
+    assert all(torch.equal(a, c) for a, c in zip(want, held))
