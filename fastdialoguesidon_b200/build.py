@@ -1,9 +1,11 @@
-"""Build recipe for the in-tree native library ``_lib/libfds_b200.so``.
+"""Build recipe for the in-tree native library ``_lib/libfds_b200.so`` and the
+Python extension ``_lib/_fds_torch.so``.
 
-One nvcc invocation, sm_100a only (``-gencode arch=compute_100a,code=sm_100a``),
-static cudart, no torch headers: the library is a plain C ABI
-(``include/fds_b200.h``) that any FFI can load. The built ``.so`` lives inside
-the package directory so that it travels with the source tree.
+The library: nvcc, sm_100a only (``-gencode arch=compute_100a,code=sm_100a``),
+static cudart, no torch headers: a plain C ABI (``include/fds_b200.h``) that any
+FFI can load. The extension (``csrc/torch_shim.cpp``, g++, torch's headers)
+checks the layer ops' tensors and calls that ABI. Both live inside the package
+directory so that they travel with the source tree.
 """
 
 from __future__ import annotations
@@ -20,8 +22,10 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libfds_b200.so"
+SHIM_PATH = LIB_DIR / "_fds_torch.so"
 INCLUDE_DIR = REPO_DIR / "include"
 
+SHIM_SOURCE = "torch_shim.cpp"
 SOURCES = ["fds_capi.cu", "fds_rope_static.cu", "fds_int8.cu", "fds_norm.cu", "fds_window.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -46,16 +50,16 @@ def nvcc_path() -> str:
 
 
 def _inputs() -> list[Path]:
-    files = [CSRC / s for s in SOURCES]
-    files += sorted(CSRC.glob("*.cuh"))
+    files = [CSRC / s for s in (*SOURCES, SHIM_SOURCE)]
+    files += sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
     files += sorted(INCLUDE_DIR.glob("*.h"))
     return files
 
 
 def is_stale() -> bool:
-    if not LIB_PATH.exists():
+    if not (LIB_PATH.exists() and SHIM_PATH.exists()):
         return True
-    mtime = LIB_PATH.stat().st_mtime
+    mtime = min(LIB_PATH.stat().st_mtime, SHIM_PATH.stat().st_mtime)
     return any(f.stat().st_mtime > mtime for f in _inputs())
 
 
@@ -69,7 +73,7 @@ def _run(cmd: list[str], verbose: bool) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if any source is newer than it (or ``force``)."""
+    """Compile the library and the extension if any source is newer (or ``force``)."""
     if not force and not is_stale():
         return LIB_PATH
     LIB_DIR.mkdir(parents=True, exist_ok=True)
@@ -81,17 +85,36 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return _run([nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xptxas=-v", "-Xcompiler",
                      "-fPIC,-fvisibility=hidden", "-I", str(INCLUDE_DIR), "-c", "-o", str(obj), str(CSRC / src)], verbose)
 
-    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, os.cpu_count() or 1)) as pool:
+        shim = pool.submit(_build_shim, verbose)
         log = "".join(pool.map(compile_one, zip(SOURCES, objs)))
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(tmp), *map(str, objs)], verbose)
     for obj in objs:
         obj.unlink()
+    shim.result()
     if verbose:
         sys.stdout.write(log)
     check_launch_registers(log)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
+
+
+def _build_shim(verbose: bool) -> None:
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    tmp = SHIM_PATH.with_suffix(".so.tmp")
+    _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-I", str(INCLUDE_DIR), "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+          "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
+          str(CSRC / SHIM_SOURCE), "-o", str(tmp), "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+          "-lc10_cuda"], verbose)
+    os.replace(tmp, SHIM_PATH)
 
 
 def check_launch_registers(ptxas_log: str) -> None:
