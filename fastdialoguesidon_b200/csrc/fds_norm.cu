@@ -1,5 +1,7 @@
-// fds_norm.cu - fds_residual_norm_fwd: argument checks, the choice of how many
-// warps share a row, and the launch.
+// fds_norm.cu - fds_residual_norm_fwd: argument checks, the shape of the CTAs,
+// and the launch.
+#include <algorithm>
+
 #include "capi_internal.h"
 #include "norm_kernel.cuh"
 
@@ -7,32 +9,50 @@ using namespace fds_detail;
 
 namespace {
 
-template <typename T, int NCH, int WPR, bool kQuant>
-int launch(const fds::norm::Params& p, cudaStream_t stream) {
-    const int per = WPR == 1 ? fds::norm::kWarpRows : 1;
-    const dim3 grid(static_cast<unsigned>((p.rows + per - 1) / per)), block(32 * (WPR == 1 ? per : WPR));
-    cudaError_t e = launch_pdl(fds::norm::residual_norm_kernel<T, NCH, WPR, kQuant>, grid, block, 0, stream, p);
+using namespace fds::norm;
+
+template <typename T, int NCH, int R, int kMode, bool kXf32, bool kQuant>
+int launch(Params& p, int threads, int per_sm, int sms, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(std::min(p.rows, sms * per_sm))), block(threads);
+    auto kern = residual_norm_kernel<T, NCH, R, kMode, kXf32, kQuant>;
+    using Rg = Ring<NCH, kMode, kXf32>;
+    static std::atomic<uint64_t> smem_set{0};
+    cudaError_t e = set_smem_once(kern, Rg::bytes(32 * kMaxWarps), smem_set);
+    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "cudaFuncSetAttribute(norm): %s", cudaGetErrorString(e));
+    e = launch_pdl(kern, grid, block, Rg::bytes(threads), stream, p);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "residual norm launch: %s", cudaGetErrorString(e));
     return FDS_OK;
 }
 
-// The fewest warps per row whose threads hold at most 4 chunks of 8 elements
-// (5 and more would leave fewer warps per SM to cover the memory latency);
-// past 4 warps x 4 chunks a row takes 8 warps and as many chunks as it needs.
-template <typename T, bool kQuant>
-int launch_shape(const fds::norm::Params& p, cudaStream_t s) {
-    const int c = p.c;
-    if (c <= 256) return launch<T, 1, 1, kQuant>(p, s);
-    if (c <= 512) return launch<T, 2, 1, kQuant>(p, s);
-    if (c <= 768) return launch<T, 3, 1, kQuant>(p, s);
-    if (c <= 1024) return launch<T, 4, 1, kQuant>(p, s);
-    if (c <= 1536) return launch<T, 3, 2, kQuant>(p, s);
-    if (c <= 2048) return launch<T, 4, 2, kQuant>(p, s);
-    if (c <= 3072) return launch<T, 3, 4, kQuant>(p, s);
-    if (c <= 4096) return launch<T, 4, 4, kQuant>(p, s);
-    if (c <= 8192) return launch<T, 4, 8, kQuant>(p, s);
-    return launch<T, 8, 8, kQuant>(p, s);
+// A CTA as wide as the row: 8 columns a thread up to 4096, 16 or 32 beyond. The
+// grid is what the SMs hold at once (16 warps each at 128 registers, 32 for the
+// quantiser at 64); four rows at a time once every CTA gets eight or more,
+// single rows below (those are bound by one row's latency).
+template <typename T, int kMode, bool kXf32, bool kQuant>
+int launch_shape(Params& p, int sms, cudaStream_t s) {
+    const int nch = p.c <= 4096 ? 1 : (p.c <= 8192 ? 2 : 4);
+    const int warps = (p.c + 256 * nch - 1) / (256 * nch);
+    const int per_sm = std::max(1, (kMode == kQuantOnly && nch == 1 ? 32 : 16) / warps);
+    if (nch == 4) return launch<T, 4, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
+    if (nch == 2) return launch<T, 2, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
+    if (p.rows >= 8 * sms * per_sm) return launch<T, 1, 4, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
+    return launch<T, 1, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
+}
+
+template <typename T, bool kXf32>
+int launch_mode(Params& p, int sms, cudaStream_t s) {
+    const bool quant = p.h_scale != nullptr;
+    if (p.y != nullptr)
+        return quant ? launch_shape<T, kBoth, kXf32, true>(p, sms, s) : launch_shape<T, kBoth, kXf32, false>(p, sms, s);
+    const bool plain = p.norm == kNone && p.w == nullptr && p.b == nullptr && p.scale == nullptr && p.shift == nullptr;
+    if (quant && plain && !kXf32) return launch_shape<T, kQuantOnly, false, true>(p, sms, s);
+    return quant ? launch_shape<T, kNormOnly, kXf32, true>(p, sms, s) : launch_shape<T, kNormOnly, kXf32, false>(p, sms, s);
+}
+
+template <typename T>
+int launch_type(Params& p, int sms, cudaStream_t s) {
+    return p.x_f32 ? launch_mode<T, true>(p, sms, s) : launch_mode<T, false>(p, sms, s);
 }
 
 constexpr int kMaxWidth = 16384;
@@ -57,6 +77,7 @@ extern "C" int fds_residual_norm_fwd(const FdsResidualNormArgs* a, void* stream)
     if (a->y == nullptr && (a->gate != nullptr || a->post_w != nullptr || a->post_b != nullptr || a->post != FDS_NORM_NONE))
         return set_error(FDS_ERR_INVALID_ARGUMENT, "gate and the norm after the block need y");
     if (a->y != nullptr && a->x_out == nullptr) return set_error(FDS_ERR_INVALID_ARGUMENT, "null x_out pointer");
+    if (a->y == nullptr && a->x_out != nullptr) return set_error(FDS_ERR_INVALID_ARGUMENT, "x_out without y (x is not changed)");
     if (a->x_out == nullptr && a->h == nullptr) return set_error(FDS_ERR_INVALID_ARGUMENT, "neither x_out nor h is given");
     if (a->h_scale != nullptr && a->h == nullptr) return set_error(FDS_ERR_INVALID_ARGUMENT, "h_scale without h");
     const int xs = a->x_f32 ? 4 : 2, ps = a->param_f32 ? 4 : 2, hs = a->h_scale != nullptr ? 1 : 2;
@@ -85,11 +106,12 @@ extern "C" int fds_residual_norm_fwd(const FdsResidualNormArgs* a, void* stream)
     p.x_f32 = a->x_f32, p.param_f32 = a->param_f32, p.post = a->post, p.norm = a->norm;
     p.alpha = a->alpha, p.eps = a->eps;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool quant = a->h_scale != nullptr;
-    int rc;
-    if (a->dtype == FDS_DTYPE_FP16)
-        rc = quant ? launch_shape<__half, true>(p, s) : launch_shape<__half, false>(p, s);
-    else
-        rc = quant ? launch_shape<__nv_bfloat16, true>(p, s) : launch_shape<__nv_bfloat16, false>(p, s);
+    const auto wide = [&](const void* q, int64_t stride) {
+        return (reinterpret_cast<uintptr_t>(q) & 31u) == 0 && (p.rows <= 1 || stride % 8 == 0);
+    };
+    p.x_wide = wide(p.x, p.x_stride) && wide(p.x_out, p.x_out_stride);
+    const int sms = sm_count();
+    if (sms <= 0) return set_error(FDS_ERR_CUDA, "cannot query the SM count of the current device");
+    const int rc = a->dtype == FDS_DTYPE_FP16 ? launch_type<__half>(p, sms, s) : launch_type<__nv_bfloat16>(p, sms, s);
     return rc == FDS_OK ? set_ok() : rc;
 }

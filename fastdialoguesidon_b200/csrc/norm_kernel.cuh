@@ -14,10 +14,18 @@
 //
 // Bound by memory: a row is read once (x, y), held in registers through up to
 // five reductions, and written once (x', h): (2 * stream + 4) bytes per
-// element against ~14 flops. A row belongs to WPR warps whose threads hold NCH
-// chunks of 8 consecutive elements each; all of a row's loads are issued before
-// the first reduction, so a warp has NCH * 256 elements in flight. The 16-byte
-// parameter loads hit L1 / L2: a window's rows share them.
+// element against ~14 flops. A CTA is as wide as a row (a thread holds NCH
+// chunks of 8 columns) and walks a contiguous range of rows, R at a time:
+// * the vectors of a thread's columns are folded once per window into four fp32
+//   coefficients a column that stay in registers,
+//     x' = alpha * x + unit(y) * G + Gb    G = gate * post_w, Gb = gate * post_b
+//     h  = unit(x') * W + Wb               W = w (1 + scale), Wb = b (1 + scale) + shift
+//   (unit: the norm without its vectors);
+// * R rows share each reduction's shuffles and barrier;
+// * the next rows come through a ring of asynchronous copies in shared memory
+//   that each warp fills and reads by itself (no CTA barrier), so that up to
+//   192 KB per SM are in flight while the present rows pass through their
+//   reductions.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -49,6 +57,7 @@ struct Params {
     int64_t gate_stride, mod_stride;                     // elements between windows (0: shared)
     int32_t rows, c, length;  // rows per window
     int32_t x_f32, param_f32;
+    int32_t x_wide;           // fp32 rows of x and x_out on 32-byte boundaries: 256-bit accesses
     int32_t post, norm;       // Kind
     float alpha, eps;
 };
@@ -87,234 +96,411 @@ __device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]) {
     }
 }
 
-// 8 parameters from element `at` (a multiple of 8)
+// 8 parameters from element `at` (a multiple of 8), as they come from memory: a
+// vector that is absent reads nothing. Loading and converting are separate, so
+// that the loads of all vectors are in flight together.
+struct Param8 {
+    uint4 a, b;
+};
+__device__ __forceinline__ Param8 param_load(const void* p, bool f32, int64_t at) {
+    Param8 r;
+    r.a = r.b = make_uint4(0, 0, 0, 0);
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + (f32 ? 4 : 2) * at);
+    if (p != nullptr) r.a = __ldg(q);
+    if (p != nullptr && f32) r.b = __ldg(q + 1);
+    return r;
+}
 template <typename T>
-__device__ __forceinline__ void param8(const void* p, bool f32, int64_t at, float (&v)[8]) {
+__device__ __forceinline__ void param_value(const Param8& r, bool f32, bool present, float otherwise, float (&v)[8]) {
     if (f32) {
-        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-        const float4 a = __ldg(q), b = __ldg(q + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        const uint32_t u[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(u[e]);
     } else {
-        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + at)), v);
+        unpack8<T>(r.a, v);
+    }
+    if (!present) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = otherwise;
     }
 }
 
-// Sum / maximum over the WPR warps of a row; `slot` differs between the
-// reductions of one row, so one barrier each is enough.
-template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float* red, int slot) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if constexpr (WPR > 1) {
-        if ((threadIdx.x & 31) == 0) red[slot * WPR + (threadIdx.x >> 5)] = v;
-        __syncthreads();
-        v = 0.f;
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) v += red[slot * WPR + i];
+// 8 fp32 values as one 256-bit access (32-byte aligned), or as two of 128 bits
+__device__ __forceinline__ void store8(float* p, bool wide, const float (&v)[8]) {
+    if (wide) {
+        asm volatile("st.global.v8.f32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]),
+                     "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "l"(p)
+                     : "memory");
+    } else {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
-    return v;
-}
-template <int WPR>
-__device__ __forceinline__ uint32_t row_max(uint32_t v, float* red, int slot) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    if constexpr (WPR > 1) {
-        if ((threadIdx.x & 31) == 0) red[slot * WPR + (threadIdx.x >> 5)] = __uint_as_float(v);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) v = max(v, __float_as_uint(red[slot * WPR + i]));
-    }
-    return v;
 }
 
-// t <- LayerNorm / RMS norm of the row (elements past c stay 0 and count for nothing)
-template <int NCH, int WPR>
-__device__ __forceinline__ void normalise(float (&t)[NCH][8], int kind, int lane8, int c, float eps, float* red,
-                                          int slot) {
-    const float inv_c = 1.f / static_cast<float>(c);
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+    static __device__ __forceinline__ float zero() { return 0.f; }
+};
+// the larger of two non-negative floats by their bits: infinities and, above them, NaN win
+struct MaxBits {
+    __device__ __forceinline__ float operator()(float a, float b) const {
+        return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+    }
+    static __device__ __forceinline__ float zero() { return 0.f; }
+};
+
+constexpr int kSlots = 5;       // reductions per group of rows at most
+constexpr int kMaxWarps = 16;
+
+// Reduces v[r] (row r) over the CTA's threads, in place. Four rows share their
+// shuffles: after two exchanging steps each 8-lane group holds one row. `red`
+// is this reduction's own [kMaxWarps][R] block (slots alternate, so that one
+// barrier separates its writes from the previous reads).
+template <int R, typename Op>
+__device__ __forceinline__ void reduce(float (&v)[R], float* red, Op op) {
+    static_assert(R == 1 || R == 4, "one or four rows");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    float a = v[0];
+    if constexpr (R == 4) {
+        const bool hi = (lane & 16) != 0, odd = (lane & 8) != 0;
+        a = op(hi ? v[2] : v[0], __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 16));
+        const float b = op(hi ? v[3] : v[1], __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 16));
+        a = op(odd ? b : a, __shfl_xor_sync(0xffffffffu, odd ? a : b, 8));
+    } else {
+        a = op(a, __shfl_xor_sync(0xffffffffu, a, 16));
+        a = op(a, __shfl_xor_sync(0xffffffffu, a, 8));
+    }
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) a = op(a, __shfl_xor_sync(0xffffffffu, a, d));
+    if (warps == 1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = __shfl_sync(0xffffffffu, a, 8 * r);
+        return;
+    }
+    if ((lane & 7) == 0 && (lane >> 3) < R) red[warp * R + (lane >> 3)] = a;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = Op::zero();
+    for (int w = 0; w < warps; ++w) {
+        if constexpr (R == 4) {
+            const float4 t = *reinterpret_cast<const float4*>(red + 4 * w);
+            v[0] = op(v[0], t.x), v[1] = op(v[1], t.y), v[2] = op(v[2], t.z), v[3] = op(v[3], t.w);
+        } else {
+            v[0] = op(v[0], red[w]);
+        }
+    }
+}
+
+// t <- LayerNorm / RMS norm of its rows without the vectors (columns past c hold
+// 0 and count for nothing)
+template <int NCH, int R>
+__device__ __forceinline__ void unit(float (&t)[R][NCH][8], int kind, const bool (&in)[NCH], float inv_c, float eps,
+                                     float* red, int slot) {
+    float s[R];
     if (kind == kLayer) {
-        float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
+        for (int r = 0; r < R; ++r) {
+            s[r] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += t[i][e];
-        const float mean = row_sum<WPR>(s, red, slot) * inv_c;
+            for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
-            if (lane8 + i * WPR * 256 < c)
+                for (int e = 0; e < 8; ++e) s[r] += t[r][i][e];
+        }
+        reduce<R>(s, red + slot * kMaxWarps * R, Add{});
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[i][e] -= mean;
+        for (int r = 0; r < R; ++r) {
+            const float mean = s[r] * inv_c;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const float m = in[i] ? mean : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[r][i][e] -= m;
+            }
+        }
     }
-    float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
+    for (int r = 0; r < R; ++r) {
+        s[r] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(t[i][e], t[i][e], s);
-    const float r = rsqrtf(row_sum<WPR>(s, red, slot + 1) * inv_c + eps);
+        for (int i = 0; i < NCH; ++i)
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
+            for (int e = 0; e < 8; ++e) s[r] = fmaf(t[r][i][e], t[r][i][e], s[r]);
+    }
+    reduce<R>(s, red + (slot + 1) * kMaxWarps * R, Add{});
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[i][e] *= r;
+    for (int r = 0; r < R; ++r) {
+        const float k = rsqrtf(s[r] * inv_c + eps);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[r][i][e] *= k;
+    }
 }
 
-constexpr int kSlots = 5;
-constexpr int kWarpRows = 4;  // rows per CTA when a warp holds a whole row
+// What a launch computes: the rows' quantisation alone, the norm before a
+// block alone, or both sides of a block (with y).
+enum Mode : int { kQuantOnly = 0, kNormOnly = 1, kBoth = 2 };
 
-template <typename T, int NCH, int WPR, bool kQuant>
-__global__ void __launch_bounds__(WPR == 1 ? 32 * kWarpRows : 32 * WPR) residual_norm_kernel(const Params p) {
-    __shared__ float red[kSlots * WPR];
+// Ring depth in rows, and the 16-byte pieces of a row's chunk (x, then y).
+template <int NCH, int kMode, bool kXf32>
+struct Ring {
+    static constexpr int kPieces = (kXf32 ? 2 : 1) + (kMode == kBoth ? 1 : 0);
+    static constexpr int kRows = 8 / NCH;  // at most 192 KB per SM
+    static constexpr int bytes(int threads) { return kRows * NCH * kPieces * 16 * threads; }
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
+    const int4 v = ld_shared_v4(addr);
+    return make_uint4(static_cast<uint32_t>(v.x), static_cast<uint32_t>(v.y), static_cast<uint32_t>(v.z),
+                      static_cast<uint32_t>(v.w));
+}
+
+// G, Gb of chunk column `at` (1 and 0 where a vector is absent)
+template <typename T>
+__device__ __forceinline__ void block_coefficients(const Params& p, int64_t window, int at, float (&G)[8], float (&Gb)[8]) {
+    const bool pf = p.param_f32 != 0;
+    const Param8 w = param_load(p.post_w, pf, at), b = param_load(p.post_b, pf, at),
+                 g = param_load(p.gate, pf, window * p.gate_stride + at);
+    float v[8];
+    param_value<T>(w, pf, p.post_w != nullptr, 1.f, G);
+    param_value<T>(b, pf, p.post_b != nullptr, 0.f, Gb);
+    param_value<T>(g, pf, p.gate != nullptr, 1.f, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) G[e] *= v[e], Gb[e] *= v[e];
+}
+// W, Wb likewise
+template <typename T>
+__device__ __forceinline__ void norm_coefficients(const Params& p, int64_t window, int at, float (&W)[8], float (&Wb)[8]) {
+    const bool pf = p.param_f32 != 0;
+    const Param8 w = param_load(p.w, pf, at), b = param_load(p.b, pf, at),
+                 s = param_load(p.scale, pf, window * p.mod_stride + at), t = param_load(p.shift, pf, window * p.mod_stride + at);
+    float v[8];
+    param_value<T>(w, pf, p.w != nullptr, 1.f, W);
+    param_value<T>(b, pf, p.b != nullptr, 0.f, Wb);
+    param_value<T>(s, pf, p.scale != nullptr, 0.f, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) W[e] = fmaf(W[e], v[e], W[e]), Wb[e] = fmaf(Wb[e], v[e], Wb[e]);
+    param_value<T>(t, pf, p.shift != nullptr, 0.f, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) Wb[e] += v[e];
+}
+
+template <typename T, int NCH, int R, int kMode, bool kXf32, bool kQuant>
+__global__ void __launch_bounds__(32 * kMaxWarps, kMode == kQuantOnly && NCH == 1 ? 2 : 1)
+    residual_norm_kernel(const Params p) {
+    using Rg = Ring<NCH, kMode, kXf32>;
+    constexpr bool kKeep = NCH < 4;  // coefficients in registers; the widest rows read them again per group
+    static_assert((Rg::kRows & (Rg::kRows - 1)) == 0 && Rg::kRows >= R, "ring rows");
+    __shared__ __align__(16) float red_all[2 * kSlots * kMaxWarps * R];
+    extern __shared__ __align__(16) uint8_t ring_raw[];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int row = WPR == 1 ? static_cast<int>(blockIdx.x) * kWarpRows + static_cast<int>(threadIdx.x >> 5)
-                             : static_cast<int>(blockIdx.x);
-    if (row >= p.rows) return;  // whole warps of a one-warp-per-row CTA only
-    const int lane8 = 8 * static_cast<int>(WPR == 1 ? threadIdx.x & 31 : threadIdx.x);  // first element of chunk 0
-    const int64_t window = row / p.length;
-    const bool pf = p.param_f32 != 0;
-
-    float x[NCH][8];
-    {
-        uint4 ry[NCH];
-        if (p.y != nullptr) {
-            const T* y = static_cast<const T*>(p.y) + row * p.y_stride;
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int at = lane8 + i * WPR * 256;
-                ry[i] = at < p.c ? *reinterpret_cast<const uint4*>(y + at) : make_uint4(0, 0, 0, 0);
-            }
-        }
-        if (p.x_f32) {
-            const float* xr = static_cast<const float*>(p.x) + row * p.x_stride;
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int at = lane8 + i * WPR * 256;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-                if (at < p.c) {
-                    a = *reinterpret_cast<const float4*>(xr + at);
-                    b = *reinterpret_cast<const float4*>(xr + at + 4);
-                }
-                x[i][0] = a.x, x[i][1] = a.y, x[i][2] = a.z, x[i][3] = a.w;
-                x[i][4] = b.x, x[i][5] = b.y, x[i][6] = b.z, x[i][7] = b.w;
-            }
-        } else {
-            const T* xr = static_cast<const T*>(p.x) + row * p.x_stride;
-            uint4 rx[NCH];
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int at = lane8 + i * WPR * 256;
-                rx[i] = at < p.c ? *reinterpret_cast<const uint4*>(xr + at) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) unpack8<T>(rx[i], x[i]);
-        }
-        if (p.y != nullptr) {
-            float y[NCH][8];
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) unpack8<T>(ry[i], y[i]);
-            if (p.post != kNone) normalise<NCH, WPR>(y, p.post, lane8, p.c, p.eps, red, 0);
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int at = lane8 + i * WPR * 256;
-                if (at >= p.c) continue;
-                float v[8];
-                if (p.post_w != nullptr) {
-                    param8<T>(p.post_w, pf, at, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[i][e] *= v[e];
-                }
-                if (p.post_b != nullptr) {
-                    param8<T>(p.post_b, pf, at, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[i][e] += v[e];
-                }
-                if (p.gate != nullptr) {
-                    param8<T>(p.gate, pf, window * p.gate_stride + at, v);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[i][e] *= v[e];
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = fmaf(p.alpha, x[i][e], y[i][e]);
-            }
-        }
-    }
-    if (p.x_out != nullptr) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int at = lane8 + i * WPR * 256;
-            if (at >= p.c) continue;
-            const float(&v)[8] = x[i];
-            if (p.x_f32) {
-                float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.x_out) + row * p.x_out_stride + at);
-                o[0] = make_float4(v[0], v[1], v[2], v[3]);
-                o[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<T*>(p.x_out) + row * p.x_out_stride + at) =
-                    make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-            }
-        }
-    }
-    if (p.h == nullptr) return;
-
-    if (p.norm != kNone) normalise<NCH, WPR>(x, p.norm, lane8, p.c, p.eps, red, 2);
+    const int row_begin = static_cast<int>(static_cast<int64_t>(p.rows) * blockIdx.x / gridDim.x);
+    const int row_end = static_cast<int>(static_cast<int64_t>(p.rows) * (blockIdx.x + 1) / gridDim.x);
+    const float inv_c = 1.f / static_cast<float>(p.c);
+    int at[NCH];
+    bool in[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int at = lane8 + i * WPR * 256;
-        if (at >= p.c) continue;
-        float v[8];
-        if (p.w != nullptr) {
-            param8<T>(p.w, pf, at, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] *= v[e];
-        }
-        if (p.b != nullptr) {
-            param8<T>(p.b, pf, at, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] += v[e];
-        }
-        if (p.scale != nullptr) {
-            param8<T>(p.scale, pf, window * p.mod_stride + at, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = fmaf(x[i][e], v[e], x[i][e]);
-        }
-        if (p.shift != nullptr) {
-            param8<T>(p.shift, pf, window * p.mod_stride + at, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] += v[e];
-        }
-        if constexpr (!kQuant)
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.h_stride + at) =
-                make_uint4(pack2<T>(x[i][0], x[i][1]), pack2<T>(x[i][2], x[i][3]), pack2<T>(x[i][4], x[i][5]),
-                           pack2<T>(x[i][6], x[i][7]));
+        at[i] = 8 * static_cast<int>(threadIdx.x + i * blockDim.x);
+        in[i] = at[i] < p.c;
     }
-    if constexpr (kQuant) {
-        // max|h| as unsigned bits: orders the finite values, and infinities and
-        // NaN above them all
-        uint32_t m = 0;
+    // chunk i of ring row s: x's 16 or 32 bytes a thread, then y's 16. An fp32
+    // chunk is copied in 16-byte pieces that are contiguous over the lanes (whole
+    // sectors) and read as each thread's 32 bytes, so the lanes of a warp hand
+    // pieces to one another.
+    const uint32_t ring = smem_u32(ring_raw), step = 16u * blockDim.x;
+    const auto chunk = [&](int s, int i) { return ring + ((s * NCH + i) * Rg::kPieces) * step; };
+    const uint32_t unit0 = 2 * (threadIdx.x & ~31u) + (threadIdx.x & 31);  // fp32: this thread copies pieces unit0, unit0 + 32
+    // the next row to fetch; this thread's addresses walk with it
+    int next = row_begin;
+    const char* fx = static_cast<const char*>(p.x) +
+                     (static_cast<int64_t>(row_begin) * p.x_stride + (kXf32 ? 4 * unit0 : at[0])) * (kXf32 ? 4 : 2);
+    const char* fy = static_cast<const char*>(p.y) + (static_cast<int64_t>(row_begin) * p.y_stride + at[0]) * 2;
+    const int64_t fx_step = p.x_stride * (kXf32 ? 4 : 2), fy_step = p.y_stride * 2;
+    const auto fetch = [&]() {  // one commit group per row, empty past the end
+        if (next < row_end) {
+            const int s = (next - row_begin) & (Rg::kRows - 1);
 #pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(fabsf(x[i][e])));
-        m = row_max<WPR>(m, red, 4);
-        const float big = __uint_as_float(m);
-        // a row with an infinity or a NaN gets the scale NaN (its products say so);
-        // one whose 127 / max could overflow is zero to every 16-bit reader
-        const bool finite = m < 0x7f800000u, tiny = big < 7.888609e-31f;  // 2^-100
-        const float inv = finite && !tiny ? __fdiv_rn(127.f, big) : 0.f;
-        const float s = finite ? (tiny ? 0.f : __fdiv_rn(big, 127.f)) : __uint_as_float(0x7fffffffu);
-        if (lane8 == 0) p.h_scale[row] = s;
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int at = lane8 + i * WPR * 256;
-            if (at >= p.c) continue;
-            // rint(h * inv) from the 1.5 * 2^23 shifter: the low byte of the sum's
-            // bits is the integer (|h * inv| <= 127; the product is rounded first, as
-            // a separate multiply and rint would)
-            uint32_t u[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(x[i][e], inv), 12582912.f));
-            const uint32_t lo = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-            const uint32_t hi = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
-            *reinterpret_cast<uint2*>(static_cast<int8_t*>(p.h) + row * p.h_stride + at) = make_uint2(lo, hi);
+            for (int i = 0; i < NCH; ++i) {
+                const int first = 8 * i * static_cast<int>(blockDim.x);  // the chunk's first column
+                if constexpr (kXf32) {
+                    const char* g = fx + static_cast<int64_t>(first) * 4;
+                    const int col = first + 4 * static_cast<int>(unit0);
+                    if (col < p.c) copy16(chunk(s, i) + 16u * unit0, g);
+                    if (col + 128 < p.c) copy16(chunk(s, i) + 16u * (unit0 + 32), g + 512);
+                } else if (in[i]) {
+                    copy16(chunk(s, i) + 16u * threadIdx.x, fx + static_cast<int64_t>(first) * 2);
+                }
+                if constexpr (kMode == kBoth)
+                    if (in[i])
+                        copy16(chunk(s, i) + (Rg::kPieces - 1) * step + 16u * threadIdx.x, fy + static_cast<int64_t>(first) * 2);
+            }
         }
+        copy_commit();
+        ++next;
+        fx += fx_step;
+        fy += fy_step;
+    };
+#pragma unroll
+    for (int r = 0; r < Rg::kRows; ++r) fetch();
+
+    char* ox = static_cast<char*>(p.x_out) + (static_cast<int64_t>(row_begin) * p.x_out_stride + at[0]) * (kXf32 ? 4 : 2);
+    char* oh = static_cast<char*>(p.h) + (static_cast<int64_t>(row_begin) * p.h_stride + at[0]) * (kQuant ? 1 : 2);
+    const int64_t ox_step = p.x_out_stride * (kXf32 ? 4 : 2), oh_step = p.h_stride * (kQuant ? 1 : 2);
+    float G[kKeep ? NCH : 1][8], Gb[kKeep ? NCH : 1][8], W[kKeep ? NCH : 1][8], Wb[kKeep ? NCH : 1][8];
+    int window = 0, window_end = 0, parity = 0;
+    for (int this_row = row_begin; this_row < row_end;) {
+        if (this_row >= window_end) {
+            window = this_row / p.length;
+            window_end = p.rows - window * p.length > p.length ? (window + 1) * p.length : p.rows;
+            if constexpr (kKeep && kMode != kQuantOnly) {
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    if (in[i]) {
+                        if constexpr (kMode == kBoth) block_coefficients<T>(p, window, at[i], G[i], Gb[i]);
+                        norm_coefficients<T>(p, window, at[i], W[i], Wb[i]);
+                    } else {  // columns past c stay 0
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) G[i][e] = Gb[i][e] = W[i][e] = Wb[i][e] = 0.f;
+                    }
+                }
+            }
+        }
+        const int this_n = min(R, min(row_end, window_end) - this_row);  // a group's rows are of one window
+        const int slot = this_row - row_begin;
+        copy_wait<Rg::kRows - R>();
+        __syncwarp();
+        const auto load_x = [&](int r, int i, float (&v)[8]) {
+            const bool on = in[i] && r < this_n;
+            const int s = (slot + r) & (Rg::kRows - 1);
+            const uint32_t from = chunk(s, i) + (kXf32 ? 32u : 16u) * threadIdx.x;
+            const uint4 a = on ? ld_shared_u4(from) : make_uint4(0, 0, 0, 0);
+            if constexpr (kXf32) {
+                const uint4 b = on ? ld_shared_u4(from + 16) : make_uint4(0, 0, 0, 0);
+                const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(u[e]);
+            } else {
+                unpack8<T>(a, v);
+            }
+        };
+        float x[R][NCH][8];
+        float* red = red_all + parity * kSlots * kMaxWarps * R;
+        parity ^= 1;
+        if constexpr (kMode == kBoth) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const bool on = in[i] && r < this_n;
+                    const uint32_t from =
+                        chunk((slot + r) & (Rg::kRows - 1), i) + (Rg::kPieces - 1) * step + 16u * threadIdx.x;
+                    unpack8<T>(on ? ld_shared_u4(from) : make_uint4(0, 0, 0, 0), x[r][i]);
+                }
+            if (p.post != kNone) unit<NCH, R>(x, p.post, in, inv_c, p.eps, red, 0);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    if constexpr (!kKeep) {
+                        if (!in[i]) continue;
+                        block_coefficients<T>(p, window, at[i], G[0], Gb[0]);
+                    }
+                    constexpr int kI = kKeep ? 1 : 0;
+                    float v[8];
+                    load_x(r, i, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        x[r][i][e] = fmaf(p.alpha, v[e], fmaf(x[r][i][e], G[kI * i][e], Gb[kI * i][e]));
+                    if (!in[i] || r >= this_n) continue;
+                    const float(&o)[8] = x[r][i];
+                    char* to = ox + r * ox_step + static_cast<int64_t>(8 * i) * blockDim.x * (kXf32 ? 4 : 2);
+                    if constexpr (kXf32)
+                        store8(reinterpret_cast<float*>(to), p.x_wide != 0, o);
+                    else
+                        *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
+                                                                   pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+                }
+            ox += this_n * ox_step;
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) load_x(r, i, x[r][i]);
+        }
+        __syncwarp();  // every lane has read its slots
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r < this_n) fetch();  // into them
+        if (p.h != nullptr) {
+            if (kMode != kQuantOnly && p.norm != kNone) unit<NCH, R>(x, p.norm, in, inv_c, p.eps, red, 2);
+            float big[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                big[r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    constexpr int kI = kKeep ? 1 : 0;
+                    if constexpr (!kKeep && kMode != kQuantOnly) {
+                        if (!in[i]) continue;
+                        norm_coefficients<T>(p, window, at[i], W[0], Wb[0]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if constexpr (kMode != kQuantOnly) x[r][i][e] = fmaf(x[r][i][e], W[kI * i][e], Wb[kI * i][e]);
+                        if constexpr (kQuant) big[r] = MaxBits{}(big[r], fabsf(x[r][i][e]));
+                    }
+                }
+            }
+            if constexpr (kQuant) reduce<R>(big, red + 4 * kMaxWarps * R, MaxBits{});
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r >= this_n) continue;
+                float inv = 0.f;
+                if constexpr (kQuant) {
+                    // a row with an infinity or a NaN gets the scale NaN (its products
+                    // say so); one whose 127 / max could overflow is zero
+                    const bool finite = __float_as_uint(big[r]) < 0x7f800000u, tiny = big[r] < 7.888609e-31f;  // 2^-100
+                    inv = finite && !tiny ? __fdiv_rn(127.f, big[r]) : 0.f;
+                    if (threadIdx.x == 0)
+                        p.h_scale[this_row + r] =
+                            finite ? (tiny ? 0.f : __fdiv_rn(big[r], 127.f)) : __uint_as_float(0x7fffffffu);
+                }
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    if (!in[i]) continue;
+                    const float(&v)[8] = x[r][i];
+                    char* to = oh + r * oh_step + static_cast<int64_t>(8 * i) * blockDim.x * (kQuant ? 1 : 2);
+                    if constexpr (kQuant) {
+                        // rint(h * inv) from the 1.5 * 2^23 shifter: the low byte of the
+                        // sum's bits is the integer (|h * inv| <= 127; the product is
+                        // rounded first, as a separate multiply and rint would)
+                        uint32_t u[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e], inv), 12582912.f));
+                        const uint32_t lo =
+                            __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+                        const uint32_t hi =
+                            __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
+                        *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+                    } else {
+                        *reinterpret_cast<uint4*>(to) = make_uint4(
+                            pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+                    }
+                }
+            }
+        }
+        oh += this_n * oh_step;
+        this_row += this_n;
     }
 }
 

@@ -315,7 +315,7 @@ FDS_API int fds_linear_int8_fwd(const FdsLinearInt8Args* args, void* stream);
  *   z = post(y) * post_w + post_b
  *   x_out = alpha * x + gate * z
  *   h = (norm(x_out) * w + b) * (1 + scale) + shift
- * Without y (NULL) x_out is x. h uses the 32-bit x_out, before its rounding to
+ * Without y (NULL) nothing is added, and x_out is absent too. h uses the 32-bit x_out, before its rounding to
  * the stream's type. With h_scale h is int8, quantised per row: h_scale = max|h| / 127,
  * q = rint(h * (127 / max|h|)) (ties to even), so FDS_NORM_NONE without y is the
  * row quantiser of fds_linear_int8_fwd; a row whose maximum is below 2^-100 is
@@ -335,7 +335,7 @@ typedef struct FdsResidualNormArgs {
     int64_t x_stride;         /* elements; rows 16-byte aligned, likewise below */
     const void* y;            /* device, dtype, [rows, y_stride], or NULL */
     int64_t y_stride;
-    void* x_out;              /* device, x's type; or NULL without y */
+    void* x_out;              /* device, x's type; NULL without y */
     int64_t x_out_stride;
     void* h;                  /* device, dtype (int8 with h_scale), or NULL */
     int64_t h_stride;
