@@ -655,12 +655,14 @@ struct RowSoftmax {
     int i, kv_end, lane, t_begin;
     float m_run, l_run;
     uint32_t s_parity, pv_parity;
-    int w_first, w_lo, w_hi;  // kMaskWindow: columns c < w_first and w_lo <= c < w_hi of the tile are seen
+    int w_a, w_z, w_lo, w_hi;  // kMaskWindow: columns [w_a, w_z) and [w_lo, w_hi) of the tile are seen
+    bool w_whole;              // ... all of them by every row of the warp
 
     // kBand: per-score relative bias gathered from qrow (any tile; needed for
     // the near-diagonal ones); otherwise the per-row constant cb (a tile whose
     // every pair saturates the clamp, or no bias). kMask: the keys excluded
-    // (MaskKind). A row that has seen no key yet keeps m_run = -inf, l_run = 0.
+    // (MaskKind). With kMaskWindow a row may have seen no key yet: m_run stays
+    // -inf, and what it adds to O and l_run is scaled by 0 at its first key.
     template <bool kBand, int kMask>
     __device__ __forceinline__ bool step(int j, float cb) {
         bool ok = warp_wait(s_full, s_parity, ctl, err);
@@ -698,10 +700,16 @@ struct RowSoftmax {
             mult = 1.f;
             cb = 0.f;
         }
-        if constexpr (kMask == kMaskWindow) {
+        // (a branch in the one step rather than a step of its own: a second copy of
+        // the unrolled step does not fit the instruction cache beside the first)
+        if (kMask == kMaskWindow && !w_whole) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t seen = low_bits(w_first - 32 * k) | (low_bits(w_hi - 32 * k) & ~low_bits(w_lo - 32 * k));
+                // rows of a warp are neighbours: an edge crosses one or two of its
+                // four 32-column groups, the others need no selects
+                const uint32_t seen = (low_bits(w_z - 32 * k) & ~low_bits(w_a - 32 * k)) |
+                                      (low_bits(w_hi - 32 * k) & ~low_bits(w_lo - 32 * k));
+                if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
                     if ((seen & (1u << c)) == 0) s[32 * k + c] = -INFINITY;
@@ -733,7 +741,6 @@ struct RowSoftmax {
             alpha = ex2_approx(m_run - tile_max);  // 0 on the item's first tile
             m_run = tile_max;
         }
-        // (a row whose every key so far is excluded: 0, so that its exponentials are 0)
         const float add = kMask == kMaskWindow && m_run == -INFINITY ? 0.f : cb - m_run;
         const float ky = mult * (1.0f / kPolySpan), kb = (add - kPolyLo) * (1.0f / kPolySpan);
 
@@ -769,7 +776,7 @@ struct RowSoftmax {
                 warp_arrive(p_half, lane);
             }
             float2 pp;
-            if (kMask != kMaskWindow && poly_pair<kRelBias>(c)) {  // (the polynomial is > 0 at -inf)
+            if (poly_pair<kRelBias>(c)) {
                 pp = exp2_poly2(s[2 * c], s[2 * c + 1], ky, kb);
             } else {
                 const float2 x = ffma2(make_float2(s[2 * c], s[2 * c + 1]), mult2, add2);

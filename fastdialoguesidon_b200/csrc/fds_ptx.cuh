@@ -298,6 +298,31 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
     return v;
 }
 
+// Launch control: asks to cancel the launch of a CTA of this grid that has not
+// started; the 16-byte answer lands at `dst` and completes on `bar` (which
+// expects 16 bytes).
+__device__ __forceinline__ void launch_control_ask(uint32_t dst, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst),
+                 "r"(bar)
+                 : "memory");
+}
+// Whether a CTA was cancelled -- its work is the asker's now -- and its blockIdx.x.
+__device__ __forceinline__ bool launch_control_answer(uint32_t src, int& block_x) {
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+        : "=r"(got), "=r"(x)
+        : "r"(src)
+        : "memory");
+    if (got != 0) block_x = static_cast<int>(x);
+    return got != 0;
+}
+
 // Arrive on an mbarrier given by its shared::cluster address (any CTA of the cluster).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");

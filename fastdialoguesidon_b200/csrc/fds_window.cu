@@ -86,6 +86,7 @@ int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream)
     const int64_t tiles = (most_keys(p, fds::kBlockM) + fds::kBlockN - 1) / fds::kBlockN;
     int split = 1;
     while (split < fds::window::kMaxSplit && units * split * 2 <= 2 * sms && tiles >= 4 * split) split *= 2;
+    p.units = static_cast<int32_t>(units);
     if (units * split > 0x7fffffffLL) return set_error(FDS_ERR_INVALID_ARGUMENT, "too many query tiles");
     auto kern = fds::window::window_tile_kernel<T>;
     static std::atomic<uint64_t> smem_set{0};

@@ -8,22 +8,19 @@
 //
 // Two kernels, chosen by the number of query rows that share a key head:
 //
-// * window_tile_kernel: tensor cores, one CTA per 128 query rows of a (window,
-//   head), walking 128-column tiles over the union of the keys its rows see.
-//   The columns are the sinks before the union's window part, rounded up to 8
-//   (one swizzle atom), then the window part, packed: a tile may hold both, so
-//   the sinks cost their own columns and not a tile of their own. The first
-//   column of the window part is the first key that the CTA's first row sees
-//   (TMA rows start anywhere), which leaves at most two partly seen tiles per
-//   end. A tile that every row of a warp sees whole runs the mask-free step.
-//   The step is the bidirectional attention's (attn_kernel.cuh RowSoftmax); a
-//   CTA has one query tile and half an SM (128 + 128 threads, 256 TMEM
-//   columns, 98 KB), because a window is a handful of tiles: the start and
-//   the epilogue of one CTA run under the tiles of its neighbour, and a
-//   128-row tile overlaps fewer keys that its rows do not see than a 256-row
-//   unit. With few query tiles and many key tiles the column tiles of a unit
-//   are dealt to a cluster of up to 8 CTAs, whose partial (O, max, sum) are
-//   merged through distributed shared memory in rank order.
+// * window_tile_kernel: tensor cores, a unit of 128 query rows of a (window,
+//   head) at a time, walking 128-column tiles over the union of the keys its rows
+//   see. The columns are the union's window part, from the first key its first
+//   row sees on (TMA rows start anywhere), rounded up to 8 (one swizzle atom),
+//   then the sinks before it, packed: a tile may hold both, so the sinks cost
+//   their own columns and not a tile of their own, and at most one tile at the
+//   left edge and two at the right are seen in part. The step is the
+//   bidirectional attention's (attn_kernel.cuh RowSoftmax). A CTA has one query
+//   tile and half an SM (128 + 128 threads, 256 TMEM columns, 98 KB): a window is
+//   a handful of tiles, and a 128-row tile overlaps fewer keys that its rows do
+//   not see than a 256-row unit. With few query tiles and many key tiles the
+//   column tiles of a unit are dealt to a cluster of up to 8 CTAs, whose partial
+//   (O, max, sum) are merged through distributed shared memory in rank order.
 // * window_step_kernel: up to 8 query rows per key head (a decoding step):
 //   bound by reading the keys and values once. 8 lanes hold a key's 64
 //   values, 16 keys run abreast in a CTA, and the keys of a unit are dealt to a
@@ -61,6 +58,7 @@ struct Params {
     int32_t heads, kv_heads, q_len, k_len;
     int32_t left, right, sinks;
     int32_t row_blocks;  // ceil(q_len / 128)
+    int32_t units;       // batch * heads * row_blocks
     float scale_log2;
 };
 
@@ -73,10 +71,11 @@ __device__ __forceinline__ int key_end(const Params& p, int b) {
     return p.kv_len != nullptr ? min(max(p.kv_len[b], 0), p.k_len) : p.k_len;
 }
 
-// The columns of a unit of query positions [p0, p1]: keys [0, n_sink), padded
-// to s8 columns (a multiple of 8), then keys [begin, begin + n_win).
+// The columns of a unit of `rows` query rows: keys [begin, begin + n_win), padded
+// to s0 columns (a multiple of 8, where sinks follow), then keys [0, n_sink).
 struct Columns {
-    int p0, kv_end, n_sink, s8, begin, n_win;
+    int p0, kv_end, begin, n_win, s0, n_sink;
+    Columns() = default;
     __device__ __forceinline__ Columns(const Params& p, int b, int row0, int rows) {
         p0 = first_position(p, b) + row0;
         kv_end = key_end(p, b);
@@ -87,17 +86,17 @@ struct Columns {
             begin = 0;
             n_sink = 0;
         }
-        s8 = (n_sink + 7) & ~7;
         n_win = max(0, end - begin);
+        s0 = n_sink > 0 ? (n_win + 7) & ~7 : n_win;
     }
-    __device__ __forceinline__ int total() const { return s8 + n_win; }
+    __device__ __forceinline__ int total() const { return s0 + n_sink; }
 };
 
 // ---------------------------------------------------------------- tile kernel
 
 constexpr int kTileThreads = 256;
 constexpr int kTileRegs = 128;  // per thread at launch: 65536 / (2 CTAs x 256)
-constexpr int kSoftmaxRegs = 208, kControlRegs = 48;
+constexpr int kSoftmaxRegs = 200, kControlRegs = 56;
 static_assert(128 * kSoftmaxRegs + 128 * kControlRegs <= kTileThreads * kTileRegs, "register split exceeds the launch pool");
 constexpr int kKStages = 3, kVStages = 2;
 constexpr int kMaxSplit = 8;
@@ -117,10 +116,16 @@ struct TileSmem {
     static constexpr int kPHalf = kSFree + 1;
     static constexpr int kPFull = kPHalf + 1;
     static constexpr int kPvDone = kPFull + 1;
-    static constexpr int kDrain = kPvDone + 1;
-    static constexpr int kNumBars = kDrain + 1;
+    static constexpr int kQEmpty = kPvDone + 1;
+    static constexpr int kDrain = kQEmpty + 1;
+    static constexpr int kRecFull = kDrain + 1;     // [record] laid out
+    static constexpr int kRecEmpty = kRecFull + 2;  // [record] read by every role
+    static constexpr int kNext = kRecEmpty + 2;     // the next unit's launch-control answer landed
+    static constexpr int kNumBars = kNext + 1;
     static constexpr int misc = bars + kNumBars * 8;  // the bounded waits' block (attn_kernel.cuh Smem::misc)
-    static constexpr int total = misc + 48;
+    static constexpr int records = (misc + 48 + 15) / 16 * 16;
+    static constexpr int answer = records + 2 * 64;
+    static constexpr int total = answer + 16;
     static constexpr int alloc = total + 1024;
     // a split unit's partial rows, [66][128] floats (64 of O, max, sum), over the K ring
     static constexpr int part = k;
@@ -134,24 +139,6 @@ struct Maps {
     CUtensorMap q, k, v;    // boxes of 128 rows
     CUtensorMap k8, v8;     // boxes of 8 rows (tiles that hold sinks and window keys)
 };
-
-// Columns [x0, x0 + 128) of the unit's keys or values into `dst` (128 rows of
-// 128 bytes, 16384 bytes in all; rows past the tensor read as zero).
-__device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap* map, const CUtensorMap* map8, uint32_t bar,
-                                             const Columns& c, int x0, int head, int b) {
-    mbar_arrive_expect_tx(bar, kTileBytes);
-    if (x0 >= c.s8) {
-        tma_load_4d(dst, map, bar, 0, head, c.begin + x0 - c.s8, b);
-    } else if (x0 + kBlockN <= c.s8) {
-        tma_load_4d(dst, map, bar, 0, head, x0, b);
-    } else {
-#pragma unroll 1
-        for (int r = 0; r < kBlockN; r += 8) {
-            const int x = x0 + r;
-            tma_load_4d(dst + r * 128, map8, bar, 0, head, x < c.s8 ? x : c.begin + x - c.s8, b);
-        }
-    }
-}
 
 // Merge of a split unit: CTA `rank` of the cluster takes rows [128 rank / split,
 // 128 (rank + 1) / split), `split` threads a row; parts are folded in rank
@@ -193,6 +180,79 @@ __device__ __forceinline__ void merge_parts(uint32_t part, int split, int rank, 
     }
 }
 
+// A unit (row block fastest, then head, then window) and this CTA's share of
+// its tiles, [t0, t1).
+struct Unit {
+    int b, h, row0, rows, t0, t1;
+    Columns c;
+};
+
+__device__ __forceinline__ Unit make_unit(const Params& p, int unit, int split, int rank) {
+    const int bh = unit / p.row_blocks;
+    Unit u;
+    u.b = bh / p.heads;
+    u.h = bh - u.b * p.heads;
+    u.row0 = (unit - bh * p.row_blocks) * kBlockM;
+    u.rows = min(kBlockM, p.q_len - u.row0);
+    u.c = Columns(p, u.b, u.row0, u.rows);
+    const int tiles = (u.c.total() + kBlockN - 1) / kBlockN;
+    const int per = (tiles + split - 1) / split;
+    u.t0 = min(tiles, rank * per);
+    u.t1 = min(tiles, u.t0 + per);
+    return u;
+}
+
+// The units of a CTA are laid out by warp 3 ahead of the roles that use them
+// (divisions and the loads of q_start and kv_len stay off their paths), as 64-byte
+// records in a ring: {b, h, row0, rows}, {t0, t1, p0, kv_end}, {begin, n_win, s0,
+// n_sink}, {key head, tile with padding columns, tile with columns past the end,
+// more} (tiles counted from t0, -1: none; more = 0 ends the list).
+constexpr int kRecords = 2;
+constexpr int kRecordReaders = 6;  // MMA, TMA, four softmax warps
+
+__device__ __forceinline__ void store_record(uint32_t at, const Unit& u, int hk) {
+    st_shared_v4(at, make_int4(u.b, u.h, u.row0, u.rows));
+    st_shared_v4(at + 16, make_int4(u.t0, u.t1, u.c.p0, u.c.kv_end));
+    st_shared_v4(at + 32, make_int4(u.c.begin, u.c.n_win, u.c.s0, u.c.n_sink));
+    const int pad = u.c.s0 > u.c.n_win ? u.c.n_win / kBlockN - u.t0 : -1;
+    const int end = u.c.total() % kBlockN != 0 ? u.c.total() / kBlockN - u.t0 : -1;
+    st_shared_v4(at + 48, make_int4(hk, pad, end, 1));
+}
+
+// Columns [x0, x0 + 128), some of them sinks, of the keys or values of a unit
+// (128 rows of 128 bytes, 16384 bytes in all; rows past the tensor read as zero).
+inline __device__ __noinline__ void load_sink_columns(uint32_t dst, const CUtensorMap* map, const CUtensorMap* map8,
+                                                      uint32_t bar, uint32_t rec, int x0) {
+    const int4 c = ld_shared_v4(rec + 32);  // begin, n_win, s0, n_sink
+    const int b = ld_shared_v4(rec).x, head = ld_shared_v4(rec + 48).x;
+    if (x0 >= c.z) {
+        tma_load_4d(dst, map, bar, 0, head, x0 - c.z, b);
+        return;
+    }
+#pragma unroll 1
+    for (int r = 0; r < kBlockN; r += 8) {
+        const int x = x0 + r;
+        tma_load_4d(dst + r * 128, map8, bar, 0, head, x < c.z ? c.x + x : x - c.z, b);
+    }
+}
+
+// Zeroes the value rows of columns that no row of the unit sees -- the window
+// part's padding and past the end -- before a product reads them (a whole warp).
+inline __device__ __noinline__ void zero_unseen(uint32_t rec, int x0, uint32_t tile, int lane) {
+    const int4 c = ld_shared_v4(rec + 32);
+    const int z0 = c.y - x0, z1 = c.z - x0, z2 = c.z + c.w - x0;
+#pragma unroll 1
+    for (int i = lane; i < kBlockN * 8; i += 32) {
+        const int r = i >> 3;
+        if ((r >= z0 && r < z1) || r >= z2) st_shared_v4(tile + 16u * i, make_int4(0, 0, 0, 0));
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// The grid has a CTA (or cluster) per unit; a CTA that finishes early takes over
+// the units of CTAs that have not started, so that the next unit's copies and
+// first scores run under the present one's last tiles and epilogue.
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __grid_constant__ Maps maps, const Params p) {
     using S = TileSmem;
@@ -204,11 +264,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
     const WaitCtl ctl{sbase + S::misc};
     const auto bar = [&](int idx) { return sbase + S::bars + 8u * idx; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t split = cluster_nctarank(), rank = cluster_ctarank();
+    const int split = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     grid_launch_dependents();
 
     if (threadIdx.x == 0) {
         mbar_init(&bars[S::kQ], 1);
+        mbar_init(&bars[S::kQEmpty], 1);
         for (int s = 0; s < kKStages; ++s) mbar_init(&bars[S::kKFull + s], 1), mbar_init(&bars[S::kKEmpty + s], 1);
         for (int s = 0; s < kVStages; ++s) mbar_init(&bars[S::kVFull + s], 1), mbar_init(&bars[S::kVEmpty + s], 1);
         mbar_init(&bars[S::kSFull], 1);
@@ -217,6 +278,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
         mbar_init(&bars[S::kPFull], 4);
         mbar_init(&bars[S::kPvDone], 1);
         mbar_init(&bars[S::kDrain], 1);
+        for (int r = 0; r < kRecords; ++r) {
+            mbar_init(&bars[S::kRecFull + r], 1);
+            mbar_init(&bars[S::kRecEmpty + r], kRecordReaders);
+        }
+        mbar_init(&bars[S::kNext], 1);
         st_shared_volatile_u32(ctl.misc + 4, 0);
         st_shared_u64(ctl.misc + 8, reinterpret_cast<uint64_t>(p.status));
         st_shared_u64(ctl.misc + 16, static_cast<uint64_t>(p.timeout_ns > 0 ? p.timeout_ns : kDefaultTimeoutNs));
@@ -239,18 +305,19 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
     grid_dependency_wait();
     const uint32_t tmem = *reinterpret_cast<uint32_t*>(smem + S::misc);
 
-    const int unit = static_cast<int>(blockIdx.x / split);
-    const int rb = unit % p.row_blocks;
-    const int bh = unit / p.row_blocks;
-    const int h = bh % p.heads, b = bh / p.heads;
-    const int hk = h / (p.heads / p.kv_heads);
-    const int row0 = rb * kBlockM;
-    const int rows = min(kBlockM, p.q_len - row0);
-    const Columns cols(p, b, row0, rows);
-    const int tiles = (cols.total() + kBlockN - 1) / kBlockN;
-    const int per = (tiles + static_cast<int>(split) - 1) / static_cast<int>(split);
-    const int t0 = min(tiles, static_cast<int>(rank) * per), t1 = min(tiles, t0 + per);  // this CTA's tiles
+    // record of this CTA's i-th unit; record_wait: it is laid out (0 on a timeout,
+    // and at the end of the list); `release` hands its slot back
+    const auto record = [&](int i) { return sbase + S::records + 64u * (i % kRecords); };
+    const auto record_wait = [&](int i, int err) {
+        return warp_wait(bar(S::kRecFull + i % kRecords), (i / kRecords) & 1, ctl, err) &&
+               ld_shared_volatile_u32(record(i) + 60) != 0;
+    };
+    const auto record_release = [&](int i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::kRecEmpty + i % kRecords));
+    };
 
+    // The two register classes never share code again (attn_kernel.cuh).
     if (warp >= 4) {
         setmaxnreg_inc<kSoftmaxRegs>();
         const int row = ((warp & 3) << 5) + lane;
@@ -270,183 +337,246 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
         rs.lane = lane;
         rs.i = 0;
         rs.kv_end = 0;
-        rs.t_begin = t0;
-        rs.m_run = -INFINITY;
-        rs.l_run = 0.f;
         rs.s_parity = 0;
         rs.pv_parity = 0;
-        // this row's columns: the sinks (or, where they lie in the window part,
-        // those of them up to p + right), and [lo, hi)
-        const int pos = cols.p0 + row;
-        const int hi = cols.s8 + min(pos + p.right + 1, cols.kv_end) - cols.begin;
-        const int lo = cols.s8 + max(pos - p.left - cols.begin, 0);
-        const int first = cols.n_sink > 0 ? cols.n_sink : min(p.sinks, hi);
         bool ok = true;
-        for (int t = t0; ok && t < t1; ++t) {
-            const int n0 = t * kBlockN;
-            rs.w_first = first - n0;
-            rs.w_lo = lo - n0;
-            rs.w_hi = hi - n0;
-            const bool whole = rs.w_first >= kBlockN || (rs.w_lo <= 0 && rs.w_hi >= kBlockN);
-            ok = __all_sync(0xffffffffu, whole) ? rs.template step<false, kMaskNone>(t, 0.f)
-                                                : rs.template step<false, kMaskWindow>(t, 0.f);
-        }
-        float o[64];
-#pragma unroll
-        for (int c = 0; c < 64; ++c) o[c] = 0.f;
-        if (ok && t1 > t0) {
-            ok = warp_wait(rs.pv_done, rs.pv_parity, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
-            if (ok) {
+        for (int i = 0; ok && record_wait(i, FDS_STATUS_TIMEOUT_SOFTMAX); ++i) {
+            const int4 un = ld_shared_v4(record(i) + 16);  // t0, t1, p0, kv_end
+            const int t1 = un.y;
+            rs.t_begin = un.x;
+            rs.m_run = -INFINITY;
+            rs.l_run = 0.f;
+            // this row's columns: [lo, hi) of the window part and the sinks, [a, z) (where
+            // they lie in the window part: those of them up to p + right)
+            const int4 c = ld_shared_v4(record(i) + 32);  // begin, n_win, s0, n_sink
+            const int pos = un.z + row;
+            const int hi = min(pos + p.right + 1, un.w) - c.x;
+            const int lo = max(pos - p.left - c.x, 0);
+            const int a = c.w > 0 ? c.z : 0, z = c.w > 0 ? c.z + c.w : min(p.sinks, hi);
+            for (int t = rs.t_begin; ok && t < t1; ++t) {
+                const int n0 = t * kBlockN;
+                rs.w_a = a - n0;
+                rs.w_z = z - n0;
+                rs.w_lo = lo - n0;
+                rs.w_hi = hi - n0;
+                rs.w_whole = __all_sync(0xffffffffu, (rs.w_lo <= 0 && rs.w_hi >= kBlockN) || (rs.w_a <= 0 && rs.w_z >= kBlockN));
+                ok = rs.template step<false, kMaskWindow>(t, 0.f);
+            }
+            const bool none = rs.m_run == -INFINITY;  // no key seen
+            float o[64];
+            if (ok && t1 > rs.t_begin) {
+                // (the next unit's first P V overwrites O only after this warpgroup's
+                // next P store, which follows this read in program order)
+                ok = warp_wait(rs.pv_done, rs.pv_parity, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
+                rs.pv_parity ^= 1;
                 tc_fence_after();
                 uint32_t ou[64];
                 tmem_ld64(rs.tO, ou);
                 tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 64; ++c) o[c] = __uint_as_float(ou[c]);
-            }
-        }
-        T* out = static_cast<T*>(p.out) + b * p.out_stride[0] + row0 * p.out_stride[1] + h * p.out_stride[2];
-        if (split == 1) {
-            if (ok && row < rows) {
-                const bool none = rs.l_run == 0.f;  // no key seen
-                if (none) {
+                for (int e = 0; e < 64; ++e) o[e] = none ? 0.f : __uint_as_float(ou[e]);
+            } else {
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) o[c] = 0.f;
-                }
-                store_row<T>(out + row * p.out_stride[1], o, none ? 1.f : 1.f / rs.l_run);
+                for (int e = 0; e < 64; ++e) o[e] = 0.f;
             }
-        } else {
-            const uint32_t part = sbase + S::part + 4u * row;
+            if (split == 1) {
+                const int4 at = ld_shared_v4(record(i));  // b, h, row0, rows: not held in registers over the tiles
+                if (ok && row < at.w)
+                    store_row<T>(static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + row) * p.out_stride[1] +
+                                     at.y * p.out_stride[2],
+                                 o, none ? 1.f : 1.f / rs.l_run);
+            } else {
+                const uint32_t part = sbase + S::part + 4u * row;
 #pragma unroll
-            for (int c = 0; c < 64; ++c) st_shared_f32(part + 512u * c, rs.l_run == 0.f ? 0.f : o[c]);
-            st_shared_f32(part + 512u * 64, rs.m_run);
-            st_shared_f32(part + 512u * 65, rs.l_run);
+                for (int e = 0; e < 64; ++e) st_shared_f32(part + 512u * e, o[e]);
+                st_shared_f32(part + 512u * 64, rs.m_run);
+                st_shared_f32(part + 512u * 65, none ? 0.f : rs.l_run);
+            }
+            if (split == 1) record_release(i);
         }
         __syncwarp();
         tc_fence_before();
         named_barrier_sync(1, kTileThreads);
         if (split > 1) {
             cluster_sync_all();
-            merge_parts<T>(sbase + S::part, static_cast<int>(split), static_cast<int>(rank),
-                           static_cast<int>(threadIdx.x) - 128, rows, out, p.out_stride[1]);
+            const int4 at = ld_shared_v4(record(0));  // (the end of the list is in the other slot)
+            merge_parts<T>(sbase + S::part, split, rank, static_cast<int>(threadIdx.x) - 128, at.w,
+                           static_cast<T*>(p.out) + at.x * p.out_stride[0] + at.z * p.out_stride[1] + at.y * p.out_stride[2],
+                           p.out_stride[1]);
             __syncwarp();
             cluster_sync_all();  // no CTA leaves while its parts are read
         }
     } else {
         setmaxnreg_dec<kControlRegs>();
-        if (warp == 0 && t1 > t0) {
+        if (warp == 0) {
             // ------------------------------------------------ MMA issuer
             constexpr int fmt = DTypeTraits<T>::kFormat;
             constexpr uint32_t idesc_qk = idesc_f16(kBlockM, kBlockN, fmt, 0, 0);
             constexpr uint32_t idesc_pv = idesc_f16(kBlockM, kHeadDim, fmt, 0, 1);
             constexpr int err = FDS_STATUS_TIMEOUT_MMA;
-            const auto issue_s = [&](int j) {
+            int g = 0, q = 0;  // tiles and units so far (ring stages and barrier phases run on)
+            bool ok = true;
+            // S columns <- Q K(tile g)^T, once the previous scores are read out; the unit's last also frees Q
+            const auto scores = [&](int gt, bool last) {
+                if (gt > 0) ok = warp_wait(bar(S::kSFree), (gt - 1) & 1, ctl, err);
+                if (ok) ok = warp_wait(bar(S::kKFull + gt % kKStages), (gt / kKStages) & 1, ctl, err);
+                if (!ok) return;
+                tc_fence_after();
                 if (elect_one()) {
-                    const uint64_t dq = sw128_desc(sbase + S::q), dk = sw128_desc(sbase + S::k + (j % kKStages) * kTileBytes);
+                    const uint64_t dq = sw128_desc(sbase + S::q), dk = sw128_desc(sbase + S::k + (gt % kKStages) * kTileBytes);
 #pragma unroll
                     for (int k = 0; k < kHeadDim / 16; ++k) mma_ss(tmem, dq + 2 * k, dk + 2 * k, idesc_qk, k > 0);
                     mma_commit(bar(S::kSFull));
-                    mma_commit(bar(S::kKEmpty + j % kKStages));
+                    mma_commit(bar(S::kKEmpty + gt % kKStages));
+                    if (last) mma_commit(bar(S::kQEmpty));
                 }
                 __syncwarp();
             };
-            const auto issue_pv = [&](int j, int half) {
+            // O (+)= P V(tile g) over half of the tile's keys
+            const auto values = [&](int gt, int half, bool accumulate) {
+                tc_fence_after();
                 if (elect_one()) {
-                    const uint64_t dv = sw128_desc(sbase + S::v + (j % kVStages) * kTileBytes);
+                    const uint64_t dv = sw128_desc(sbase + S::v + (gt % kVStages) * kTileBytes);
 #pragma unroll
                     for (int k = 0; k < kBlockN / 32; ++k) {
                         const int kk = half * (kBlockN / 32) + k;
-                        mma_ts(tmem + kTO, tmem + kTP + 8 * kk, dv + 128 * kk, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                        mma_ts(tmem + kTO, tmem + kTP + 8 * kk, dv + 128 * kk, idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
                     }
                     if (half == 1) {
                         mma_commit(bar(S::kPvDone));
-                        mma_commit(bar(S::kVEmpty + j % kVStages));
+                        mma_commit(bar(S::kVEmpty + gt % kVStages));
                     }
                 }
                 __syncwarp();
             };
-            const int n = t1 - t0;
-            bool issued = false;
-            bool ok = warp_wait(bar(S::kQ), 0, ctl, err) && warp_wait(bar(S::kKFull), 0, ctl, err);
-            if (ok) {
-                tc_fence_after();
-                issue_s(0);
-                issued = true;
-            }
-            for (int j = 0; ok && j < n; ++j) {
-                if (j + 1 < n) {
-                    ok = warp_wait(bar(S::kSFree), j & 1, ctl, err) &&
-                         warp_wait(bar(S::kKFull + (j + 1) % kKStages), ((j + 1) / kKStages) & 1, ctl, err);
+            for (int i = 0; ok && record_wait(i, err); ++i) {
+                const uint32_t rec = record(i);
+                const int4 tiles = ld_shared_v4(rec + 16), zero = ld_shared_v4(rec + 48);
+                const int n = tiles.y - tiles.x;
+                if (n <= 0) {
+                    record_release(i);
+                    continue;
+                }
+                ok = warp_wait(bar(S::kQ), q & 1, ctl, err);
+                ++q;
+                if (ok) scores(g, n == 1);
+                for (int j = 0; ok && j < n; ++j, ++g) {
+                    if (j + 1 < n) scores(g + 1, j + 2 == n);
+                    if (ok) ok = warp_wait(bar(S::kVFull + g % kVStages), (g / kVStages) & 1, ctl, err);
                     if (!ok) break;
-                    tc_fence_after();
-                    issue_s(j + 1);
+                    if (j == zero.y || j == zero.z)
+                        zero_unseen(rec, (tiles.x + j) * kBlockN, sbase + S::v + (g % kVStages) * kTileBytes, lane);
+                    ok = warp_wait(bar(S::kPHalf), g & 1, ctl, err);
+                    if (!ok) break;
+                    values(g, 0, j > 0);
+                    ok = warp_wait(bar(S::kPFull), g & 1, ctl, err);
+                    if (!ok) break;
+                    values(g, 1, true);
                 }
-                ok = warp_wait(bar(S::kVFull + j % kVStages), (j / kVStages) & 1, ctl, err);
-                if (!ok) break;
-                // value rows of columns that no row sees: the sinks' padding and past the end
-                const int x0 = (t0 + j) * kBlockN;
-                const int z0 = max(cols.n_sink - x0, 0), z1 = min(cols.s8 - x0, kBlockN), z2 = max(cols.total() - x0, 0);
-                if (z0 < z1 || z2 < kBlockN) {
-                    const uint32_t vs = sbase + S::v + (j % kVStages) * kTileBytes;
-                    for (int i = lane; i < kBlockN * 8; i += 32) {
-                        const int r = i >> 3;
-                        if ((r >= z0 && r < z1) || r >= z2) st_shared_v4(vs + 16u * i, make_int4(0, 0, 0, 0));
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
-                ok = warp_wait(bar(S::kPHalf), j & 1, ctl, err);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(j, 0);
-                ok = warp_wait(bar(S::kPFull), j & 1, ctl, err);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(j, 1);
+                record_release(i);
             }
-            if (issued) {  // every MMA issued completes before TMEM is released
+            if (q > 0) {  // every MMA issued completes before TMEM is released
                 if (elect_one()) mma_commit(bar(S::kDrain));
                 __syncwarp();
                 wait_bounded(bar(S::kDrain), 0, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
                 __syncwarp();
             }
-        } else if (warp == 1 && t1 > t0) {
+        } else if (warp == 1) {
             // ------------------------------------------------ TMA producer
             constexpr int err = FDS_STATUS_TIMEOUT_LOAD;
-            if (elect_one()) {
-                mbar_arrive_expect_tx(bar(S::kQ), kTileBytes);
-                tma_load_4d(sbase + S::q, &maps.q, bar(S::kQ), 0, h, row0, b);
-            }
-            __syncwarp();
-            const int n = t1 - t0;
-            int nk = 0, nv = 0;  // tiles issued
+            int nk = 0, nv = 0, nq = 0;  // copies issued
             bool ok = true;
-            for (int j = 0; j < n; ++j) {
-                const int sk = j % kKStages, sv = j % kVStages;
-                if (j >= kKStages) ok = warp_wait(bar(S::kKEmpty + sk), (j / kKStages - 1) & 1, ctl, err);
-                if (!ok) break;
-                if (elect_one())
-                    load_columns(sbase + S::k + sk * kTileBytes, &maps.k, &maps.k8, bar(S::kKFull + sk), cols,
-                                 (t0 + j) * kBlockN, hk, b);
-                __syncwarp();
-                ++nk;
-                if (j >= kVStages) ok = warp_wait(bar(S::kVEmpty + sv), (j / kVStages - 1) & 1, ctl, err);
-                if (!ok) break;
-                if (elect_one())
-                    load_columns(sbase + S::v + sv * kTileBytes, &maps.v, &maps.v8, bar(S::kVFull + sv), cols,
-                                 (t0 + j) * kBlockN, hk, b);
-                __syncwarp();
-                ++nv;
+            for (int i = 0; ok && record_wait(i, err); ++i) {
+                const uint32_t rec = record(i);
+                const int4 at = ld_shared_v4(rec), tiles = ld_shared_v4(rec + 16), c = ld_shared_v4(rec + 32);  // begin, n_win, s0, n_sink
+                const int hk = ld_shared_v4(rec + 48).x;
+                if (tiles.y > tiles.x) {
+                    if (nq > 0) ok = warp_wait(bar(S::kQEmpty), (nq - 1) & 1, ctl, err);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar(S::kQ), kTileBytes);
+                        tma_load_4d(sbase + S::q, &maps.q, bar(S::kQ), 0, at.y, at.z, at.x);
+                    }
+                    __syncwarp();
+                    ++nq;
+                }
+                for (int t = tiles.x; t < tiles.y; ++t) {
+                    const int x0 = t * kBlockN, key = c.x + x0;
+                    const bool plain = c.w == 0 || x0 + kBlockN <= c.z;  // no sinks in the tile: keys from `key` on
+                    const int sk = nk % kKStages, sv = nv % kVStages;
+                    if (nk >= kKStages) ok = warp_wait(bar(S::kKEmpty + sk), (nk / kKStages - 1) & 1, ctl, err);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar(S::kKFull + sk), kTileBytes);
+                        if (plain)
+                            tma_load_4d(sbase + S::k + sk * kTileBytes, &maps.k, bar(S::kKFull + sk), 0, hk, key, at.x);
+                        else
+                            load_sink_columns(sbase + S::k + sk * kTileBytes, &maps.k, &maps.k8, bar(S::kKFull + sk), rec, x0);
+                    }
+                    __syncwarp();
+                    ++nk;
+                    if (nv >= kVStages) ok = warp_wait(bar(S::kVEmpty + sv), (nv / kVStages - 1) & 1, ctl, err);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar(S::kVFull + sv), kTileBytes);
+                        if (plain)
+                            tma_load_4d(sbase + S::v + sv * kTileBytes, &maps.v, bar(S::kVFull + sv), 0, hk, key, at.x);
+                        else
+                            load_sink_columns(sbase + S::v + sv * kTileBytes, &maps.v, &maps.v8, bar(S::kVFull + sv), rec, x0);
+                    }
+                    __syncwarp();
+                    ++nv;
+                }
+                record_release(i);
             }
             if (!ok) {
                 // aborted: the copies already issued land before the CTA exits
-                wait_bounded(bar(S::kQ), 0, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
+                if (nq > 0) wait_bounded(bar(S::kQ), (nq - 1) & 1, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
                 for (int s = 0; s < kKStages; ++s)
                     if (nk > s)
                         wait_bounded(bar(S::kKFull + s), ((nk - 1 - s) / kKStages) & 1, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
                 for (int s = 0; s < kVStages; ++s)
                     if (nv > s)
                         wait_bounded(bar(S::kVFull + s), ((nv - 1 - s) / kVStages) & 1, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
+                __syncwarp();
+            }
+        } else if (warp == 3) {
+            // ------------------------------------------------ unit records
+            // This CTA's own unit, then the units of CTAs that have not started:
+            // launch control hands them out as they are asked for, so SMs of
+            // different speeds share the units as if each had its own CTA.
+            constexpr int err = FDS_STATUS_TIMEOUT_LOAD;
+            int unit = static_cast<int>(blockIdx.x) / split;
+            bool ok = true, more = true;
+            for (int i = 0; ok; ++i) {
+                if (i >= kRecords) ok = warp_wait(bar(S::kRecEmpty + i % kRecords), (i / kRecords - 1) & 1, ctl, err);
+                if (!ok) break;
+                if (more) {
+                    const Unit un = make_unit(p, unit, split, rank);
+                    if (lane == 0) store_record(record(i), un, un.h / (p.heads / p.kv_heads));
+                } else if (lane == 0) {
+                    st_shared_volatile_u32(record(i) + 60, 0);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(S::kRecFull + i % kRecords));
+                if (!more) break;
+                if (split > 1) {  // a cluster holds one unit
+                    more = false;
+                    continue;
+                }
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar(S::kNext), 16);
+                    launch_control_ask(sbase + S::answer, bar(S::kNext));
+                }
+                __syncwarp();
+                ok = warp_wait(bar(S::kNext), i & 1, ctl, err);
+                if (!ok) {  // (the answer still lands before the CTA exits)
+                    wait_bounded(bar(S::kNext), i & 1, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
+                    __syncwarp();
+                    break;
+                }
+                more = launch_control_answer(sbase + S::answer, unit);
+                fence_proxy_async_smem();  // the answer is read before the next one is written
                 __syncwarp();
             }
         }
