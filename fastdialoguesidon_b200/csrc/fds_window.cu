@@ -42,10 +42,10 @@ cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, int block, size_t 
     return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
-// [batch, len, heads, 64] of any strides: boxes of one head x `rows` rows,
-// 128-byte swizzle, zero fill past the last row.
+// [batch, len, heads, 64] of any strides: boxes of `rows` rows x `pack` heads (the
+// heads of a row next to each other), 128-byte swizzle, zero fill past the last row.
 int make_heads_map(CUtensorMap* map, const void* base, int dtype, int heads, int len, int batch, const int64_t* stride,
-                   int rows) {
+                   int rows, int pack = 1) {
     EncodeTiledFn enc = encode_fn();
     if (enc == nullptr) return set_error(FDS_ERR_TENSOR_MAP, "cuTensorMapEncodeTiled unavailable from the driver");
     const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(len),
@@ -54,7 +54,7 @@ int make_heads_map(CUtensorMap* map, const void* base, int dtype, int heads, int
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(heads > 1 ? 2 * stride[2] : 128),
                                    static_cast<cuuint64_t>(len > 1 ? 2 * stride[1] : 128),
                                    static_cast<cuuint64_t>(batch > 1 ? 2 * stride[0] : 128)};
-    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(rows), 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(pack), static_cast<cuuint32_t>(rows), 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUtensorMapDataType dt =
         dtype == FDS_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -71,22 +71,25 @@ int64_t most_keys(const Params& p, int rows) {
 
 template <typename T>
 int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream) {
+    // the heads of a key head share units, so that its keys are read once for them
+    const int group = p.heads / p.kv_heads;
+    p.pack = group <= fds::kBlockM ? group : 1;
+    p.queries = fds::kBlockM / p.pack;
     fds::window::Maps maps;
     int rc;
-    if ((rc = make_heads_map(&maps.q, a->q, a->dtype, p.heads, p.q_len, a->batch, p.q_stride, fds::kBlockM)) != FDS_OK ||
+    if ((rc = make_heads_map(&maps.q, a->q, a->dtype, p.heads, p.q_len, a->batch, p.q_stride, p.queries, p.pack)) != FDS_OK ||
         (rc = make_heads_map(&maps.k, a->k, a->dtype, p.kv_heads, p.k_len, a->batch, p.k_stride, fds::kBlockN)) != FDS_OK ||
         (rc = make_heads_map(&maps.v, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, fds::kBlockN)) != FDS_OK ||
         (rc = make_heads_map(&maps.k8, a->k, a->dtype, p.kv_heads, p.k_len, a->batch, p.k_stride, 8)) != FDS_OK ||
         (rc = make_heads_map(&maps.v8, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, 8)) != FDS_OK)
         return rc;
-    p.row_blocks = (p.q_len + fds::kBlockM - 1) / fds::kBlockM;
-    const int64_t units = static_cast<int64_t>(a->batch) * p.heads * p.row_blocks;
+    p.row_blocks = (p.q_len + p.queries - 1) / p.queries;
+    const int64_t units = static_cast<int64_t>(a->batch) * (p.heads / p.pack) * p.row_blocks;
     // A unit's tiles are dealt to a cluster while that still fills idle SMs
     // (two CTAs each) and leaves every CTA two tiles.
-    const int64_t tiles = (most_keys(p, fds::kBlockM) + fds::kBlockN - 1) / fds::kBlockN;
+    const int64_t tiles = (most_keys(p, p.queries) + fds::kBlockN - 1) / fds::kBlockN;
     int split = 1;
     while (split < fds::window::kMaxSplit && units * split * 2 <= 2 * sms && tiles >= 4 * split) split *= 2;
-    p.units = static_cast<int32_t>(units);
     if (units * split > 0x7fffffffLL) return set_error(FDS_ERR_INVALID_ARGUMENT, "too many query tiles");
     auto kern = fds::window::window_tile_kernel<T>;
     static std::atomic<uint64_t> smem_set{0};
@@ -99,17 +102,21 @@ int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream)
     return FDS_OK;
 }
 
-template <typename T, int R, bool kMulti>
+template <typename T, int kHalves, bool kMulti>
 int launch_step(const Params& p, int batch, int sms, cudaStream_t stream) {
-    // The keys of a (window, key head) are dealt to a cluster while that leaves
-    // every CTA a full round of its 16 groups x 4 keys and at most 4 CTAs per SM.
+    // The keys of a (window, key head) are dealt to the warps of a cluster while
+    // that leaves every warp a block of 32 keys and at most 2 CTAs per SM.
     const int64_t units = static_cast<int64_t>(batch) * p.kv_heads, keys = most_keys(p, p.q_len);
     int split = 1;
-    while (split < fds::window::kMaxSplit && units * split * 2 <= 4 * sms && keys >= 128 * split) split *= 2;
-    cudaError_t e = launch_cluster(fds::window::window_step_kernel<T, R, kMulti>,
-                                   dim3(static_cast<unsigned>(split), static_cast<unsigned>(p.kv_heads),
-                                        static_cast<unsigned>(batch)),
-                                   fds::window::kStepThreads, 0, split, stream, p);
+    while (split < fds::window::kMaxSplit && units * split * 2 <= 2 * sms &&
+           keys >= 2 * split * fds::window::kStepWarps * fds::window::kStepKeys)
+        split *= 2;
+    auto kern = fds::window::window_step_kernel<T, kHalves, kMulti>;
+    static std::atomic<uint64_t> smem_set{0};
+    cudaError_t e = set_smem_once(kern, fds::window::kStepSmem, smem_set);
+    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "cudaFuncSetAttribute(window step): %s", cudaGetErrorString(e));
+    e = launch_cluster(kern, dim3(static_cast<unsigned>(split), static_cast<unsigned>(p.kv_heads), static_cast<unsigned>(batch)),
+                       fds::window::kStepThreads, fds::window::kStepSmem, split, stream, p);
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "window attention launch: %s", cudaGetErrorString(e));
     return FDS_OK;
@@ -118,15 +125,8 @@ int launch_step(const Params& p, int batch, int sms, cudaStream_t stream) {
 template <typename T>
 int launch_step_rows(const Params& p, int batch, int sms, cudaStream_t s) {
     const int rows = p.q_len * (p.heads / p.kv_heads);
-    if (p.q_len == 1) {
-        if (rows == 1) return launch_step<T, 1, false>(p, batch, sms, s);
-        if (rows == 2) return launch_step<T, 2, false>(p, batch, sms, s);
-        if (rows <= 4) return launch_step<T, 4, false>(p, batch, sms, s);
-        return launch_step<T, 8, false>(p, batch, sms, s);
-    }
-    if (rows == 2) return launch_step<T, 2, true>(p, batch, sms, s);
-    if (rows <= 4) return launch_step<T, 4, true>(p, batch, sms, s);
-    return launch_step<T, 8, true>(p, batch, sms, s);
+    if (p.q_len == 1) return rows <= 8 ? launch_step<T, 1, false>(p, batch, sms, s) : launch_step<T, 2, false>(p, batch, sms, s);
+    return rows <= 8 ? launch_step<T, 1, true>(p, batch, sms, s) : launch_step<T, 2, true>(p, batch, sms, s);
 }
 
 bool strides_ok(const void* base, const int64_t* st, int batch, int len, int heads) {

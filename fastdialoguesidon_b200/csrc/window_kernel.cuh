@@ -8,9 +8,10 @@
 //
 // Two kernels, chosen by the number of query rows that share a key head:
 //
-// * window_tile_kernel: tensor cores, a unit of 128 query rows of a (window,
-//   head) at a time, walking 128-column tiles over the union of the keys its rows
-//   see. The columns are the union's window part, from the first key its first
+// * window_tile_kernel: tensor cores, a unit of 128 query rows of a window at a
+//   time -- the queries of one head, or 128 / group queries of all the heads that
+//   share a key head, interleaved -- walking 128-column tiles over the union of
+//   the keys its rows see. The columns are the union's window part, from the first key its first
 //   row sees on (TMA rows start anywhere), rounded up to 8 (one swizzle atom),
 //   then the sinks before it, packed: a tile may hold both, so the sinks cost
 //   their own columns and not a tile of their own, and at most one tile at the
@@ -21,16 +22,18 @@
 //   not see than a 256-row unit. With few query tiles and many key tiles the
 //   column tiles of a unit are dealt to a cluster of up to 8 CTAs, whose partial
 //   (O, max, sum) are merged through distributed shared memory in rank order.
-// * window_step_kernel: up to 8 query rows per key head (a decoding step):
-//   bound by reading the keys and values once. 8 lanes hold a key's 64
-//   values, 16 keys run abreast in a CTA, and the keys of a unit are dealt to a
-//   cluster of up to 8 CTAs merged the same way.
+// * window_step_kernel: up to 16 query rows per key head (a decoding step):
+//   bound by reading the keys and values once. Each warp streams its share of the
+//   keys through a shared-memory ring of its own and multiplies them with the
+//   rows as warp-level 16 x 8 x 16 products (a 128-row tcgen05 tile would be
+//   seven-eighths empty, and the products are not what bounds it); the shares --
+//   4 warps of up to 8 CTAs of a cluster -- are merged the same way.
 //
 // Keys and values that no row of a unit sees may hold anything (a cache's
 // unwritten rows): their scores are replaced, and their value rows are zeroed
 // in shared memory before the P V product reads them (0 times an infinity
-// would not be 0). The tile kernel does multiply a value row that one row of
-// the tile sees by the zero weights of the rows that do not.
+// would not be 0), or not read at all. A value row that one row of the unit sees
+// is multiplied by the zero weights of the rows that do not.
 #pragma once
 
 #include <cuda.h>
@@ -57,8 +60,10 @@ struct Params {
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];  // elements: batch, row, head
     int32_t heads, kv_heads, q_len, k_len;
     int32_t left, right, sinks;
-    int32_t row_blocks;  // ceil(q_len / 128)
-    int32_t units;       // batch * heads * row_blocks
+    // tile kernel: `pack` heads of a unit (those of one key head, or 1) and
+    // `queries` = 128 / pack of each; row r of a unit is query r / pack, head r % pack
+    int32_t pack, queries;
+    int32_t row_blocks;  // ceil(q_len / queries)
     float scale_log2;
 };
 
@@ -140,14 +145,12 @@ struct Maps {
     CUtensorMap k8, v8;     // boxes of 8 rows (tiles that hold sinks and window keys)
 };
 
-// Merge of a split unit: CTA `rank` of the cluster takes rows [128 rank / split,
-// 128 (rank + 1) / split), `split` threads a row; parts are folded in rank
-// order, so the result does not depend on their timing.
+// Merge of row `row` of a split unit, the `part_idx`-th of `split` column ranges, into
+// `out` (the row's 64 values) if it is a real row; parts are folded in rank order,
+// so the result does not depend on their timing.
 template <typename T>
-__device__ __forceinline__ void merge_parts(uint32_t part, int split, int rank, int tid, int rows, T* out,
-                                            int64_t out_stride) {
-    const int row = rank * (kBlockM / split) + tid / split;
-    const int width = kHeadDim / split, c0 = (tid % split) * width;  // this thread's columns: 32, 16 or 8
+__device__ __forceinline__ void merge_parts(uint32_t part, int split, int row, int part_idx, bool real, T* out) {
+    const int width = kHeadDim / split, c0 = part_idx * width;  // this thread's columns: 32, 16 or 8
     float m = -INFINITY;
     for (int r = 0; r < split; ++r) m = fmaxf(m, ld_cluster_f32(map_to_rank(part + 512u * 64 + 4u * row, r)));
     float l = 0.f, f[kMaxSplit];
@@ -173,28 +176,28 @@ __device__ __forceinline__ void merge_parts(uint32_t part, int split, int rank, 
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = fmaf(ld_cluster_f32(at + 512u * (c + e)), f[r], acc[e]);
         }
-        if (row < rows)
-            *reinterpret_cast<uint4*>(out + row * out_stride + c) =
+        if (real)
+            *reinterpret_cast<uint4*>(out + c) =
                 make_uint4(norm::pack2<T>(acc[0] * inv, acc[1] * inv), norm::pack2<T>(acc[2] * inv, acc[3] * inv),
                            norm::pack2<T>(acc[4] * inv, acc[5] * inv), norm::pack2<T>(acc[6] * inv, acc[7] * inv));
     }
 }
 
-// A unit (row block fastest, then head, then window) and this CTA's share of
-// its tiles, [t0, t1).
+// A unit (row block fastest, then head group, then window): queries [row0, row0 +
+// n) of heads [h, h + pack) of window b, and this CTA's share of its tiles, [t0, t1).
 struct Unit {
-    int b, h, row0, rows, t0, t1;
+    int b, h, row0, n, t0, t1;
     Columns c;
 };
 
 __device__ __forceinline__ Unit make_unit(const Params& p, int unit, int split, int rank) {
-    const int bh = unit / p.row_blocks;
+    const int groups = p.heads / p.pack, bg = unit / p.row_blocks;
     Unit u;
-    u.b = bh / p.heads;
-    u.h = bh - u.b * p.heads;
-    u.row0 = (unit - bh * p.row_blocks) * kBlockM;
-    u.rows = min(kBlockM, p.q_len - u.row0);
-    u.c = Columns(p, u.b, u.row0, u.rows);
+    u.b = bg / groups;
+    u.h = (bg - u.b * groups) * p.pack;
+    u.row0 = (unit - bg * p.row_blocks) * p.queries;
+    u.n = min(p.queries, p.q_len - u.row0);
+    u.c = Columns(p, u.b, u.row0, u.n);
     const int tiles = (u.c.total() + kBlockN - 1) / kBlockN;
     const int per = (tiles + split - 1) / split;
     u.t0 = min(tiles, rank * per);
@@ -204,14 +207,14 @@ __device__ __forceinline__ Unit make_unit(const Params& p, int unit, int split, 
 
 // The units of a CTA are laid out by warp 3 ahead of the roles that use them
 // (divisions and the loads of q_start and kv_len stay off their paths), as 64-byte
-// records in a ring: {b, h, row0, rows}, {t0, t1, p0, kv_end}, {begin, n_win, s0,
+// records in a ring: {b, h, row0, n}, {t0, t1, p0, kv_end}, {begin, n_win, s0,
 // n_sink}, {key head, tile with padding columns, tile with columns past the end,
 // more} (tiles counted from t0, -1: none; more = 0 ends the list).
 constexpr int kRecords = 2;
 constexpr int kRecordReaders = 6;  // MMA, TMA, four softmax warps
 
 __device__ __forceinline__ void store_record(uint32_t at, const Unit& u, int hk) {
-    st_shared_v4(at, make_int4(u.b, u.h, u.row0, u.rows));
+    st_shared_v4(at, make_int4(u.b, u.h, u.row0, u.n));
     st_shared_v4(at + 16, make_int4(u.t0, u.t1, u.c.p0, u.c.kv_end));
     st_shared_v4(at + 32, make_int4(u.c.begin, u.c.n_win, u.c.s0, u.c.n_sink));
     const int pad = u.c.s0 > u.c.n_win ? u.c.n_win / kBlockN - u.t0 : -1;
@@ -321,6 +324,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
     if (warp >= 4) {
         setmaxnreg_inc<kSoftmaxRegs>();
         const int row = ((warp & 3) << 5) + lane;
+        const int query = row / p.pack, head = row - query * p.pack;  // of this row in its unit
         const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
         RowSoftmax<T, false> rs;
         rs.tS = tmem + lane_addr;
@@ -349,7 +353,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
             // this row's columns: [lo, hi) of the window part and the sinks, [a, z) (where
             // they lie in the window part: those of them up to p + right)
             const int4 c = ld_shared_v4(record(i) + 32);  // begin, n_win, s0, n_sink
-            const int pos = un.z + row;
+            const int pos = un.z + query;
             const int hi = min(pos + p.right + 1, un.w) - c.x;
             const int lo = max(pos - p.left - c.x, 0);
             const int a = c.w > 0 ? c.z : 0, z = c.w > 0 ? c.z + c.w : min(p.sinks, hi);
@@ -380,10 +384,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
                 for (int e = 0; e < 64; ++e) o[e] = 0.f;
             }
             if (split == 1) {
-                const int4 at = ld_shared_v4(record(i));  // b, h, row0, rows: not held in registers over the tiles
-                if (ok && row < at.w)
-                    store_row<T>(static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + row) * p.out_stride[1] +
-                                     at.y * p.out_stride[2],
+                const int4 at = ld_shared_v4(record(i));  // b, h, row0, n: not held in registers over the tiles
+                if (ok && query < at.w)
+                    store_row<T>(static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + query) * p.out_stride[1] +
+                                     (at.y + head) * p.out_stride[2],
                                  o, none ? 1.f : 1.f / rs.l_run);
             } else {
                 const uint32_t part = sbase + S::part + 4u * row;
@@ -400,9 +404,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
         if (split > 1) {
             cluster_sync_all();
             const int4 at = ld_shared_v4(record(0));  // (the end of the list is in the other slot)
-            merge_parts<T>(sbase + S::part, split, rank, static_cast<int>(threadIdx.x) - 128, at.w,
-                           static_cast<T*>(p.out) + at.x * p.out_stride[0] + at.z * p.out_stride[1] + at.y * p.out_stride[2],
-                           p.out_stride[1]);
+            // CTA `rank` takes rows [128 rank / split, ..), `split` threads a row
+            const int tid = static_cast<int>(threadIdx.x) - 128;
+            const int mrow = rank * (kBlockM / split) + tid / split, mq = mrow / p.pack;
+            merge_parts<T>(sbase + S::part, split, mrow, tid % split, mq < at.w,
+                           static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + mq) * p.out_stride[1] +
+                               (at.y + mrow - mq * p.pack) * p.out_stride[2]);
             __syncwarp();
             cluster_sync_all();  // no CTA leaves while its parts are read
         }
@@ -494,7 +501,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
                     if (nq > 0) ok = warp_wait(bar(S::kQEmpty), (nq - 1) & 1, ctl, err);
                     if (!ok) break;
                     if (elect_one()) {
-                        mbar_arrive_expect_tx(bar(S::kQ), kTileBytes);
+                        mbar_arrive_expect_tx(bar(S::kQ), static_cast<uint32_t>(p.pack * p.queries) * 128u);
                         tma_load_4d(sbase + S::q, &maps.q, bar(S::kQ), 0, at.y, at.z, at.x);
                     }
                     __syncwarp();
@@ -596,191 +603,233 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
 
 // ---------------------------------------------------------------- step kernel
 
-constexpr int kStepThreads = 128;
-constexpr int kStepRows = 8;     // query rows per key head at most
-constexpr int kStepUnroll = 4;   // keys per 8-lane group in flight
+constexpr int kStepWarps = 4;
+constexpr int kStepThreads = 32 * kStepWarps;
+constexpr int kStepRows = 16;     // query rows per key head at most: one m16 fragment
+constexpr int kStepKeys = 32;     // keys of a block
+constexpr int kStepStages = 3;    // blocks in a warp's ring
+constexpr int kBlockBytes = kStepKeys * 128;                       // keys or values of a block
+constexpr int kStepWarpBytes = kStepStages * 2 * kBlockBytes;
+constexpr int kStepSmem = kStepWarps * kStepWarpBytes;
+constexpr int kPartFloats = 66;   // a row's 64 of O, max, sum
+static_assert(kStepWarps * kStepRows * kPartFloats * 4 <= kStepSmem, "partial rows over the rings");
 
-// R query rows (row r: query r / group, head hk * group + r % group), R a power
-// of two >= the rows there are. kMulti: several queries, whose windows differ.
-template <typename T, int R, bool kMulti>
+// 16 bytes, or zeros, asynchronously into shared memory.
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+template <bool kTrans>
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+    if constexpr (kTrans)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+}
+
+// c += a (16 x 16, row major) * b (16 x 8, column major), fp32 accumulation
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Row r is query r / group of key head hk, head hk * group + r % group. kHalves:
+// 1 with at most 8 rows (the fragments' rows 8..15 are zero and skipped), else 2.
+// kMulti: several queries, whose windows differ. The keys of a unit go to
+// 4 * cluster warps in contiguous shares of whole blocks.
+template <typename T, int kHalves, bool kMulti>
 __global__ void __launch_bounds__(kStepThreads) window_step_kernel(const Params p) {
-    __shared__ float part[4][R][66];  // per warp: 64 of O, max, sum
+    extern __shared__ __align__(128) uint8_t step_smem[];
     grid_launch_dependents();
     grid_dependency_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane & 7;                                    // dims [8 sub, 8 sub + 8)
-    const int grp = static_cast<int>(threadIdx.x >> 3);          // 16 groups
+    const int g = lane >> 2, t = lane & 3;  // fragment row (or key, or value column) and column pair
     const int split = static_cast<int>(gridDim.x), rank = static_cast<int>(blockIdx.x);
     const int hk = blockIdx.y, b = blockIdx.z;
     const int group = p.heads / p.kv_heads;
     const int n_rows = p.q_len * group;
-    const Columns cols(p, b, 0, p.q_len);
-    const int total = cols.n_sink + cols.n_win;  // no padding here
-    const int per = (total + split - 1) / split;
-    const int x_begin = min(total, rank * per), x_end = min(total, x_begin + per);
 
-    float q[R][8];
-    int lo[R], hi[R];
+    // the query rows as A fragments, straight from memory
+    uint32_t q[4][4];
+    const T* qb = static_cast<const T*>(p.q) + b * p.q_stride[0] + 2 * t;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int rr = min(r, n_rows - 1), i = rr / group;
-        const T* src = static_cast<const T*>(p.q) + b * p.q_stride[0] + i * p.q_stride[1] +
-                       (hk * group + rr % group) * p.q_stride[2] + 8 * sub;
-        norm::unpack8<T>(*reinterpret_cast<const uint4*>(src), q[r]);
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h;
+        const bool on = h < kHalves && r < n_rows;
+        const T* src = qb + (on ? (r / group) * p.q_stride[1] + (hk * group + r % group) * p.q_stride[2] : 0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[r][e] *= p.scale_log2;
-        lo[r] = cols.p0 + i - p.left;
-        hi[r] = cols.p0 + i + p.right;
-    }
-    float m[R], l[R], acc[R][8];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[r][e] = 0.f;
-    }
-    const T* kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[2] + 8 * sub;
-    const T* vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[2] + 8 * sub;
-    for (int x0 = x_begin; x0 < x_end; x0 += 16 * kStepUnroll) {
-        uint4 kr[kStepUnroll], vr[kStepUnroll];
-        int key[kStepUnroll];
-#pragma unroll
-        for (int u = 0; u < kStepUnroll; ++u) {
-            const int x = x0 + grp + 16 * u;
-            key[u] = x < x_end ? (x < cols.n_sink ? x : cols.begin + x - cols.n_sink) : -1;
-            kr[u] = vr[u] = make_uint4(0, 0, 0, 0);
-            if (key[u] >= 0) {
-                kr[u] = __ldg(reinterpret_cast<const uint4*>(kb + key[u] * p.k_stride[1]));
-                vr[u] = __ldg(reinterpret_cast<const uint4*>(vb + key[u] * p.v_stride[1]));
-            }
-        }
-        float s[R][kStepUnroll];
-#pragma unroll
-        for (int u = 0; u < kStepUnroll; ++u) {
-            float kf[8];
-            norm::unpack8<T>(kr[u], kf);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float d = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) d = fmaf(q[r][e], kf[e], d);
-#pragma unroll
-                for (int w = 4; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
-                const bool seen = key[u] >= 0 &&
-                                  (!kMulti || (key[u] <= hi[r] && (key[u] >= lo[r] || key[u] < p.sinks)));
-                s[r][u] = seen ? d : -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float mt = m[r];
-#pragma unroll
-            for (int u = 0; u < kStepUnroll; ++u) mt = fmaxf(mt, s[r][u]);
-            const float base = mt == -INFINITY ? 0.f : mt;
-            const float alpha = ex2_approx(m[r] - base);
-            m[r] = mt;
-            l[r] *= alpha;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[r][e] *= alpha;
-#pragma unroll
-            for (int u = 0; u < kStepUnroll; ++u) {
-                s[r][u] = ex2_approx(s[r][u] - base);
-                l[r] += s[r][u];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kStepUnroll; ++u) {
-            float vf[8];
-            norm::unpack8<T>(vr[u], vf);
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (kMulti && !(key[u] <= hi[r] && (key[u] >= lo[r] || key[u] < p.sinks))) continue;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(s[r][u], vf[e], acc[r][e]);
-            }
+        for (int k = 0; k < 4; ++k) {
+            q[k][h] = on ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * k)) : 0u;
+            q[k][2 + h] = on ? __ldg(reinterpret_cast<const uint32_t*>(src + 16 * k + 8)) : 0u;
         }
     }
-    // the four groups of a warp, then the warps, then the CTAs of the unit
+
+    const Columns cols(p, b, 0, p.q_len);
+    const int total = cols.n_sink + cols.n_win;  // sinks first, unpadded
+    const int blocks = (total + kStepKeys - 1) / kStepKeys;
+    const int shares = split * kStepWarps, share = rank * kStepWarps + warp;
+    const int b_begin = static_cast<int>(static_cast<int64_t>(blocks) * share / shares);
+    const int b_end = static_cast<int>(static_cast<int64_t>(blocks) * (share + 1) / shares);
+
+    const uint32_t ring = smem_u32(step_smem) + warp * kStepWarpBytes;
+    const T* kb = static_cast<const T*>(p.k) + b * p.k_stride[0] + hk * p.k_stride[2] + 8 * (lane & 7);
+    const T* vb = static_cast<const T*>(p.v) + b * p.v_stride[0] + hk * p.v_stride[2] + 8 * (lane & 7);
+    const auto fetch = [&](int blk) {  // 8 lanes a key; 16-byte piece c of key r at c ^ (r & 7)
+        if (blk < b_end) {
+            const uint32_t dst = ring + ((blk - b_begin) % kStepStages) * 2 * kBlockBytes;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-        for (int w = 8; w < 32; w <<= 1) {
-            const float mo = __shfl_xor_sync(0xffffffffu, m[r], w), lo_ = __shfl_xor_sync(0xffffffffu, l[r], w);
-            const float mm = fmaxf(m[r], mo), base = mm == -INFINITY ? 0.f : mm;
-            const float fa = ex2_approx(m[r] - base), fb = ex2_approx(mo - base);
-            m[r] = mm;
-            l[r] = l[r] * fa + lo_ * fb;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                acc[r][e] = acc[r][e] * fa + __shfl_xor_sync(0xffffffffu, acc[r][e], w) * fb;
+            for (int i = 0; i < kStepKeys / 4; ++i) {
+                const int r = 4 * i + (lane >> 3), x = blk * kStepKeys + r;
+                const bool on = x < total;
+                const int64_t key = on ? (x < cols.n_sink ? x : cols.begin + x - cols.n_sink) : 0;
+                const uint32_t to = dst + 128u * r + 16u * ((lane & 7) ^ (r & 7));
+                copy16_or_zero(to, kb + key * p.k_stride[1], on);
+                copy16_or_zero(to + kBlockBytes, vb + key * p.v_stride[1], on);
+            }
         }
-        if (lane < 8) {
+        norm::copy_commit();
+    };
 #pragma unroll
-            for (int e = 0; e < 8; ++e) part[warp][r][8 * lane + e] = acc[r][e];
-            if (lane == 0) part[warp][r][64] = m[r], part[warp][r][65] = l[r];
+    for (int s = 0; s < kStepStages - 1; ++s) fetch(b_begin + s);
+
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+
+    for (int blk = b_begin; blk < b_end; ++blk) {
+        norm::copy_wait<kStepStages - 2>();
+        __syncwarp();  // every lane's copies of this block have landed, and the slot read last is free
+        fetch(blk + kStepStages - 1);
+        const uint32_t ks = ring + ((blk - b_begin) % kStepStages) * 2 * kBlockBytes, vs = ks + kBlockBytes;
+
+        float s[4][4];  // scores of 8-key columns n: rows g (0, 1) and g + 8 (2, 3), keys 8 n + 2 t, + 1
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {  // 32 dims: four 8 x 8 matrices, keys 8 n .. 8 n + 7
+                uint32_t f[4];
+                load_matrices<false>(f, ks + 128u * (8 * n + (lane & 7)) + 16u * ((4 * k2 + (lane >> 3)) ^ (lane & 7)));
+                mma16816<T>(s[n], q[2 * k2], f[0], f[1]);
+                mma16816<T>(s[n], q[2 * k2 + 1], f[2], f[3]);
+            }
         }
+        const int x0 = blk * kStepKeys;
+        if (kMulti || x0 + kStepKeys > total) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = x0 + 8 * n + 2 * t + (e & 1);
+                    bool seen = x < total;
+                    if constexpr (kMulti) {
+                        const int key = x < cols.n_sink ? x : cols.begin + x - cols.n_sink;
+                        const int pos = cols.p0 + (g + 8 * (e >> 1)) / group;
+                        seen = seen && key <= pos + p.right && (key >= pos - p.left || key < p.sinks);
+                    }
+                    if (!seen) s[n][e] = -INFINITY;
+                }
+        }
+        uint32_t pa[2][4];  // the weights as A fragments over 16 keys each
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pa[i][1] = pa[i][3] = 0;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            float mt = s[0][2 * h];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) mt = fmaxf(mt, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2)) * p.scale_log2;
+            const float mn = fmaxf(m[h], mt), base = mn == -INFINITY ? 0.f : mn;
+            const float alpha = ex2_approx(m[h] - base);
+            m[h] = mn;
+            l[h] *= alpha;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) o[n][2 * h] *= alpha, o[n][2 * h + 1] *= alpha;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float e0 = ex2_approx(fmaf(s[n][2 * h], p.scale_log2, -base));
+                const float e1 = ex2_approx(fmaf(s[n][2 * h + 1], p.scale_log2, -base));
+                l[h] += e0 + e1;
+                pa[n >> 1][2 * (n & 1) + h] = norm::pack2<T>(e0, e1);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int n = 0; n < 8; n += 2) {  // keys 16 i .. + 15, value columns 8 n .. + 15
+                uint32_t f[4];
+                const int r = 16 * i + (lane & 15);
+                load_matrices<true>(f, vs + 128u * r + 16u * ((n + (lane >> 4)) ^ (r & 7)));
+                mma16816<T>(o[n], pa[i], f[0], f[1]);
+                mma16816<T>(o[n + 1], pa[i], f[2], f[3]);
+            }
+    }
+
+    // this warp's rows, over the rings once every warp is done with its own
+    norm::copy_wait<0>();
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(step_smem);  // [warp][row][66]
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        float* row = part + (warp * kStepRows + g + 8 * h) * kPartFloats;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) *reinterpret_cast<float2*>(row + 8 * n + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if (t == 0) row[64] = m[h], row[65] = l[h];
     }
     __syncthreads();
-    // fold the warps into part[0] (each thread its own columns; max and sum last)
-    for (int i = threadIdx.x; i < R * 64; i += kStepThreads) {
+    if (split > 1) cluster_sync_all();
+    // merge all shares in order; the CTAs of the cluster take the rows' columns in turn
+    for (int i = rank * kStepThreads + static_cast<int>(threadIdx.x); i < n_rows * 64; i += split * kStepThreads) {
         const int r = i >> 6, c = i & 63;
+        const uint32_t at = smem_u32(part + r * kPartFloats);
         float mm = -INFINITY;
+        for (int k = 0; k < split; ++k) {
+            const uint32_t a = map_to_rank(at + 4u * 64, k);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, part[w][r][64]);
-        const float base = mm == -INFINITY ? 0.f : mm;
-        float o = 0.f, ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = ex2_approx(part[w][r][64] - base);
-            o = fmaf(part[w][r][c], f, o);
-            ll = fmaf(part[w][r][65], f, ll);
+            for (int w = 0; w < kStepWarps; ++w) mm = fmaxf(mm, ld_cluster_f32(a + 4u * w * kStepRows * kPartFloats));
         }
-        part[0][r][c] = o;
-        if (split == 1) {
-            if (r < n_rows) {
-                T* out = static_cast<T*>(p.out) + b * p.out_stride[0] + (r / group) * p.out_stride[1] +
-                         (hk * group + r % group) * p.out_stride[2];
-                out[c] = static_cast<T>(ll == 0.f ? 0.f : o / ll);
-            }
-        }
-    }
-    if (split == 1) return;
-    __syncthreads();
-    if (threadIdx.x < R) {
-        const int r = threadIdx.x;
-        float mm = -INFINITY;
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, part[w][r][64]);
         const float base = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f;
-        for (int w = 0; w < 4; ++w) ll = fmaf(part[w][r][65], ex2_approx(part[w][r][64] - base), ll);
-        part[0][r][64] = mm;
-        part[0][r][65] = ll;
-    }
-    __syncthreads();
-    cluster_sync_all();
-    // merge in rank order; the CTAs of the cluster share the rows' columns
-    for (int i = rank * kStepThreads + static_cast<int>(threadIdx.x); i < R * 64; i += split * kStepThreads) {
-        const int r = i >> 6, c = i & 63;
-        const uint32_t at = smem_u32(&part[0][r][0]);
-        float mm = -INFINITY;
-        for (int k = 0; k < split; ++k) mm = fmaxf(mm, ld_cluster_f32(map_to_rank(at + 4u * 64, k)));
-        const float base = mm == -INFINITY ? 0.f : mm;
-        float o = 0.f, ll = 0.f;
+        float acc = 0.f, sum = 0.f;
         for (int k = 0; k < split; ++k) {
             const uint32_t a = map_to_rank(at, k);
-            const float f = ex2_approx(ld_cluster_f32(a + 4u * 64) - base);
-            o = fmaf(ld_cluster_f32(a + 4u * c), f, o);
-            ll = fmaf(ld_cluster_f32(a + 4u * 65), f, ll);
+#pragma unroll
+            for (int w = 0; w < kStepWarps; ++w) {
+                const uint32_t aw = a + 4u * w * kStepRows * kPartFloats;
+                const float f = ex2_approx(ld_cluster_f32(aw + 4u * 64) - base);
+                acc = fmaf(ld_cluster_f32(aw + 4u * c), f, acc);
+                sum = fmaf(ld_cluster_f32(aw + 4u * 65), f, sum);
+            }
         }
-        if (r < n_rows) {
-            T* out = static_cast<T*>(p.out) + b * p.out_stride[0] + (r / group) * p.out_stride[1] +
-                     (hk * group + r % group) * p.out_stride[2];
-            out[c] = static_cast<T>(ll == 0.f ? 0.f : o / ll);
-        }
+        T* out = static_cast<T*>(p.out) + b * p.out_stride[0] + (r / group) * p.out_stride[1] +
+                 (hk * group + r % group) * p.out_stride[2];
+        out[c] = static_cast<T>(sum == 0.f ? 0.f : acc / sum);
     }
     __syncwarp();
-    cluster_sync_all();
+    if (split > 1) cluster_sync_all();  // no CTA leaves while its parts are read
 }
 
 }  // namespace window

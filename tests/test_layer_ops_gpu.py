@@ -94,6 +94,15 @@ def test_window_shared_key_heads_in_tiles(cuda_device):
     _check_window(q, k, v, 70, 10, 5, q_start=_i32(0, 100))
 
 
+@pytest.mark.parametrize("Lq,H,Hk", [(100, 4, 2), (90, 6, 2), (61, 5, 1), (33, 16, 2), (40, 16, 1), (9, 130, 1), (5, 12, 3), (1, 16, 1),
+                                     (1, 40, 1), (2, 24, 2)])
+@pytest.mark.parametrize("left,right,sinks", [(100, 0, 4), (40, 9, 0), (700, 0, 16)])
+def test_window_head_groups(cuda_device, Lq, H, Hk, left, right, sinks):
+    """Heads of one key head packed into a tile's rows: group sizes that divide 128, do not, and exceed it."""
+    q, k, v = _qkv(2, Lq, 800, H, Hk, torch.bfloat16, seed=Lq + H)
+    _check_window(q, k, v, left, right, sinks, q_start=_i32(800 - Lq, 350))
+
+
 @pytest.mark.parametrize("Lq", [1, 3, 150])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_window_unseen_rows_may_hold_anything(cuda_device, Lq, bad):
