@@ -32,7 +32,7 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, int esize, const void* 
 template <typename T, int BN, int kEpi, bool kPair>
 int launch(const Maps& m, const fds::gemm::Params& p, int grid, cudaStream_t stream) {
     auto kern = fds::gemm::gemm_kernel<T, BN, kEpi, kPair, true>;
-    constexpr int smem = fds::gemm::Smem<BN, kPair, kEpi == fds::gemm::kRope>::alloc;
+    constexpr int smem = fds::gemm::Smem<BN, kPair, kEpi == fds::gemm::kRope, true>::alloc;
     static std::atomic<uint64_t> smem_set{0};
     cudaError_t e = set_smem_once(kern, smem, smem_set);
     if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "cudaFuncSetAttribute(int8 gemm): %s", cudaGetErrorString(e));
@@ -96,7 +96,7 @@ int max_pairs() {
     int n = cached[dev].load(std::memory_order_relaxed);
     if (n == 0) {
         auto kern = fds::gemm::gemm_kernel<__half, 256, fds::gemm::kStore, true, true>;
-        constexpr int smem = fds::gemm::Smem<256, true>::alloc;
+        constexpr int smem = fds::gemm::Smem<256, true, false, true>::alloc;
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2);
@@ -123,24 +123,40 @@ struct Tile {
     bool pair;
 };
 
-// Of the tilings, the one whose waves over the SMs cost least. A tile costs an
-// SM its columns plus a fixed share for filling the pipeline and the epilogue
-// of the last tile.
-Tile choose_tile(int64_t m, int64_t n, int64_t sms, int64_t pairs, int want_bn, int want_pair) {
+// Of the tilings, the one that should finish first: its launch, then as many
+// waves of tiles as the SMs (pairs) need, each tile for as long as its products
+// take (they grow with k) but at least as long as its epilogue. The constants are
+// microseconds fitted to a sweep on a B200 (m 600 - 48000, n 1024 - 3072, k 256 - 4096,
+// each within 10 %): at n = 3072, m = 6000 single 256-column tiles lead below k =
+// 2048 (k = 256: 13.1 against 16.1 us, 1024: 19.5 against 20.7), pairs from there
+// on (2048: 28.5 against 31.4, 4096: 50.4 against 55.2); narrow tiles lead where
+// wide ones leave SMs idle (m = 1500, n = k = 1024: 128 columns 5.7 us, 256 6.7).
+Tile choose_tile(int64_t m, int64_t n, int64_t k, int epilogue, int64_t sms, int64_t pairs, int want_bn, int want_pair) {
+    struct Cost {
+        int bn;
+        bool pair;
+        double launch, tile, per_k, epi16, epi32;  // per_k: of 1024
+    };
+    const Cost all[] = {{256, true, 4.0, 1.2, 2.70, 3.0, 5.2},
+                        {128, true, 4.0, 0.8, 1.62, 1.9, 3.3},
+                        {256, false, 3.0, 1.2, 2.90, 2.5, 5.0},
+                        {128, false, 3.0, 0.5, 2.08, 1.35, 2.8},
+                        {64, false, 3.0, 0.3, 1.85, 0.9, 1.6}};
     Tile best{128, false};
     double best_cost = 1e30;
-    const Tile all[] = {{256, true}, {128, true}, {256, false}, {128, false}, {64, false}};
-    for (const Tile& t : all) {
-        if (want_bn != 0 && t.bn != want_bn) continue;
-        if (want_pair == FDS_GEMM_SINGLE && t.pair) continue;
-        if (want_pair == FDS_GEMM_PAIR && !t.pair) continue;
-        if (t.pair && (pairs < 1 || (m <= fds::gemm::kBM && want_pair != FDS_GEMM_PAIR))) continue;
-        const int64_t units = t.pair ? pairs : sms;
-        const int64_t tm = t.pair ? 2 * fds::gemm::kBM : fds::gemm::kBM;
-        const int64_t tiles = (m + tm - 1) / tm * ((n + t.bn - 1) / t.bn);
+    for (const Cost& c : all) {
+        if (want_bn != 0 && c.bn != want_bn) continue;
+        if (want_pair == FDS_GEMM_SINGLE && c.pair) continue;
+        if (want_pair == FDS_GEMM_PAIR && !c.pair) continue;
+        if (c.pair && (pairs < 1 || (m <= fds::gemm::kBM && want_pair != FDS_GEMM_PAIR))) continue;
+        const int64_t units = c.pair ? pairs : sms;
+        const int64_t tm = c.pair ? 2 * fds::gemm::kBM : fds::gemm::kBM;
+        const int64_t tiles = (m + tm - 1) / tm * ((n + c.bn - 1) / c.bn);
         const int64_t waves = (tiles + units - 1) / units;
-        const double cost = static_cast<double>(waves) * (t.bn + (t.pair ? 24 : 64));
-        if (cost < best_cost) best_cost = cost, best = t;
+        const double products = c.tile + c.per_k * static_cast<double>(k) / 1024.0;
+        const double cost = c.launch + static_cast<double>(waves) *
+                                           std::max(products, epilogue == FDS_EPILOGUE_ACCUMULATE_F32 ? c.epi32 : c.epi16);
+        if (cost < best_cost) best_cost = cost, best = Tile{c.bn, c.pair};
     }
     return best;
 }
@@ -203,7 +219,7 @@ extern "C" int fds_linear_int8_fwd(const FdsLinearInt8Args* a, void* stream) {
     const int64_t pairs = a->cta_pair == FDS_GEMM_SINGLE ? 0 : std::min<int64_t>(sms / 2, max_pairs());
     if (a->cta_pair == FDS_GEMM_PAIR && pairs < 1)
         return set_error(FDS_ERR_INVALID_ARGUMENT, "no CTA pair can be launched on this device");
-    const Tile t = choose_tile(a->m, a->n, sms, pairs, a->tile_n, a->cta_pair);
+    const Tile t = choose_tile(a->m, a->n, a->k, a->epilogue, sms, pairs, a->tile_n, a->cta_pair);
     const int tile_m = t.pair ? 2 * fds::gemm::kBM : fds::gemm::kBM;
     const int64_t tiles_n = (a->n + t.bn - 1) / t.bn;
     const int64_t tiles = (static_cast<int64_t>(a->m) + tile_m - 1) / tile_m * tiles_n;

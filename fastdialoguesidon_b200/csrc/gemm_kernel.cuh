@@ -25,8 +25,9 @@
 //   warp 1      MMA issuer (one elected lane; the even CTA of a pair):
 //               tcgen05.mma kind::f16, M = 128 (256 for a pair), N = BN,
 //               K = 16, fp32 accumulators in TMEM
-//   warp 2      TMEM owner (allocates / releases the 2 x BN columns)
-//   warp 3      idle
+//   warp 2      TMEM owner (allocates / releases the 2 x BN columns); 8-bit
+//               operands: the tile's column scales and biases into shared memory
+//   warp 3      RoPE: the tile's cos / sin rows
 //   warps 4-11  epilogue: thread = output row = TMEM lane; two warps per lane
 //               quarter, each taking half of the tile's columns. A warp turns
 //               128 bytes of each of its 32 rows at a time into a swizzled
@@ -62,13 +63,20 @@ enum Epi : int { kStore = 0, kRope = 1, kAccum = 2 };
 // stage while the tensor cores eat one stage per 256 / 512 cycles.
 // kCs: the RoPE epilogue's cos / sin rows of the tile (128 rows x 32 fp32 of
 // each table, 128-byte swizzle) take 32 KB from the ring.
-template <int BN, bool kPair, bool kCs = false>
+// kInt8: the tile's column scales and biases are staged too, and the ring takes
+// the rest. (A second staging box per epilogue warp, so that a box is filled
+// while the previous one is read out, cost 256-column tiles a stage and measured
+// slower: 6000 x 1024 -> 3072 at 21.0 against 19.5 us.)
+template <int BN, bool kPair, bool kCs = false, bool kInt8 = false>
 struct Smem {
     static constexpr int kBNc = kPair ? BN / 2 : BN;  // W rows this CTA loads per tile
     static constexpr int a_bytes = kBM * kRowBytes;
     static constexpr int b_bytes = kBNc * kRowBytes;
     static constexpr int kCsBytes = kCs ? 2 * kBM * 128 : 0;
-    static constexpr int kStages = (192 * 1024 - kCsBytes) / (a_bytes + b_bytes);
+    static constexpr int kColBytes = kInt8 ? BN * 6 : 0;  // a tile's w_scale (fp32) and bias (16 bits)
+    static constexpr int kRingBytes =
+        kInt8 ? 227 * 1024 - 1024 - 320 - kEpiWarps * 32 * 128 - kColBytes : 192 * 1024;
+    static constexpr int kStages = (kRingBytes - kCsBytes) / (a_bytes + b_bytes);
     static constexpr int a = 0;
     static constexpr int b = a + kStages * a_bytes;
     // one staging box per epilogue warp: 32 rows x 128 bytes, 1024-aligned (the
@@ -76,7 +84,8 @@ struct Smem {
     static constexpr int kStgBytes = 32 * 128;
     static constexpr int stg = b + kStages * b_bytes;
     static constexpr int cs = stg + kEpiWarps * kStgBytes;  // cos rows, then sin rows
-    static constexpr int bars = cs + kCsBytes;
+    static constexpr int col = cs + kCsBytes;
+    static constexpr int bars = col + kColBytes;
     static constexpr int kFull = 0;                 // [stage] A and W tiles landed (a pair: both CTAs', on the even CTA)
     static constexpr int kEmpty = kFull + kStages;  // [stage] MMAs done with the stage
     static constexpr int kAccFull = kEmpty + kStages;    // [buffer] tile's accumulator complete
@@ -84,7 +93,9 @@ struct Smem {
     static constexpr int kDrain = kAccEmpty + 2;
     static constexpr int kCsFull = kDrain + 1;   // the tile's cos / sin rows landed (or are not needed)
     static constexpr int kCsEmpty = kCsFull + 1; // every epilogue warp has its rows in registers
-    static constexpr int kNumBars = kCsEmpty + 1;
+    static constexpr int kColFull = kCsEmpty + 1;   // kInt8: the tile's column scales and biases are in place
+    static constexpr int kColEmpty = kColFull + 1;  // every epilogue warp is done with them
+    static constexpr int kNumBars = kColEmpty + 1;
     // misc block, same offsets as the attention kernel's (the bounded waits read
     // it): +0 TMEM base, +4 abort flag, +8 status pointer, +16 timeout, +32 mirror
     static constexpr int misc = bars + kNumBars * 8;
@@ -138,28 +149,19 @@ __device__ __forceinline__ float bias_at(const uint4 (&raw)[4], int c) {
     return to_f<T>(reinterpret_cast<const T*>(&raw[c >> 3])[c & 7]);
 }
 
-// The 8-bit operands' columns: w_scale[n0 + c] (c < kN) as raw 16-byte groups;
-// columns past n (a multiple of 8) read nothing and give zeros.
-template <int kN>
-__device__ __forceinline__ void fetch_scale(const float* w_scale, int n0, int n, float4 (&ws)[kN / 4]) {
-#pragma unroll
-    for (int q = 0; q < kN / 4; ++q)
-        ws[q] = n0 + 4 * q < n ? __ldg(reinterpret_cast<const float4*>(w_scale + n0) + q) : make_float4(0, 0, 0, 0);
-}
+// 8-bit operands: four columns' results from their integer sums, the row's scale
+// and the staged column scales and biases (shared memory, the same addresses in
+// every lane).
 template <typename T>
-__device__ __forceinline__ void fetch_bias_n(const T* bias, int n0, int n, uint4 (&raw)[4]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-        raw[q] = bias != nullptr && n0 + 8 * q < n ? __ldg(reinterpret_cast<const uint4*>(bias + n0) + q)
-                                                   : make_uint4(0, 0, 0, 0);
-}
-// column d's scaled sum; both scales are multiplied first, as one token's and
-// one channel's scale
-template <int kN>
-__device__ __forceinline__ float scaled(uint32_t acc, const float4 (&ws)[kN / 4], int d, float as) {
-    const float4 w = ws[d >> 2];
-    const float s = (d & 3) == 0 ? w.x : ((d & 3) == 1 ? w.y : ((d & 3) == 2 ? w.z : w.w));
-    return static_cast<float>(static_cast<int32_t>(acc)) * (as * s);
+__device__ __forceinline__ void scale4(float* y, const uint32_t* acc, float as, uint32_t scale, uint32_t bias) {
+    const float4 w = ld_shared_v4f32(scale);
+    uint32_t b[2];
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(b[0]), "=r"(b[1]) : "r"(bias) : "memory");
+    const T* bt = reinterpret_cast<const T*>(b);
+    y[0] = fmaf(static_cast<float>(static_cast<int32_t>(acc[0])), as * w.x, to_f<T>(bt[0]));
+    y[1] = fmaf(static_cast<float>(static_cast<int32_t>(acc[1])), as * w.y, to_f<T>(bt[1]));
+    y[2] = fmaf(static_cast<float>(static_cast<int32_t>(acc[2])), as * w.z, to_f<T>(bt[2]));
+    y[3] = fmaf(static_cast<float>(static_cast<int32_t>(acc[3])), as * w.w, to_f<T>(bt[3]));
 }
 
 // This lane's 128-byte row of its warp's staging box (16-byte chunk j at chunk
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_cos,
                 const __grid_constant__ CUtensorMap map_sin, const Params p) {
-    using S = Smem<BN, kPair, kEpi == kRope>;
+    using S = Smem<BN, kPair, kEpi == kRope, kInt8>;
     constexpr int kTileM = kPair ? 2 * kBM : kBM;
     constexpr int kBKe = kInt8 ? kBK8 : kBK;
     // epilogue warps with columns to write: a 64-column tile is one 64-column box per row group
@@ -221,6 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars[S::kDrain], 1);
         mbar_init(&bars[S::kCsFull], 1);
         mbar_init(&bars[S::kCsEmpty], kActiveWarps);
+        mbar_init(&bars[S::kColFull], 1);
+        mbar_init(&bars[S::kColEmpty], kActiveWarps);
         st_shared_volatile_u32(ctl.misc + 4, 0);
         st_shared_u64(ctl.misc + 8, reinterpret_cast<uint64_t>(p.status));
         st_shared_u64(ctl.misc + 16, static_cast<uint64_t>(p.timeout_ns > 0 ? p.timeout_ns : kDefaultTimeoutNs));
@@ -354,6 +358,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             wait_bounded(bar(S::kDrain), 0, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
             __syncwarp();
         }
+    } else if (warp == 2 && kInt8) {
+        // ------------------------------------------------ column scales and biases of each tile
+        int lt = 0;
+        for (int t = unit0; t < p.tiles; t += units, ++lt) {
+            // (the next tile's are in registers while the epilogue uses this one's)
+            const int n0 = (t % p.tiles_n) * BN;
+            float w[BN / 32];
+            T b[BN / 32];
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                const int c = n0 + 32 * i + lane;
+                w[i] = c < p.n ? __ldg(p.w_scale + c) : 0.f;
+                b[i] = p.bias != nullptr && c < p.n ? static_cast<const T*>(p.bias)[c] : static_cast<T>(0.f);
+            }
+            if (lt >= 1 && !warp_wait(bar(S::kColEmpty), (lt - 1) & 1, ctl, FDS_STATUS_TIMEOUT_LOAD)) break;
+            float* cw = reinterpret_cast<float*>(smem + S::col);
+            T* cb = reinterpret_cast<T*>(smem + S::col + 4 * BN);
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                cw[32 * i + lane] = w[i];
+                cb[32 * i + lane] = b[i];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(S::kColFull));
+        }
     } else if (warp == 3 && kEpi == kRope) {
         // ------------------------------------------------ cos / sin rows of each tile
         // (positions (m0 + r) % seq_len, r < 128: one TMA box of each table when
@@ -411,12 +440,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int m0 = (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM, n0 = (t % p.tiles_n) * BN;
             const int y0 = m0 + wq * 32;     // the warp's first row; rows >= m are clipped by TMA
             const bool live = y0 < p.m;      // a box wholly past the last row is not copied
-            ok = warp_wait(bar(S::kAccFull + buf), (lt >> 1) & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
+            float as = 0.f;  // 8-bit operands: this row's scale
+            if constexpr (kInt8) {
+                as = m0 + row < p.m ? __ldg(p.a_scale + m0 + row) : 0.f;
+                ok = warp_wait(bar(S::kColFull), lt & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
+            }
+            if (ok) ok = warp_wait(bar(S::kAccFull + buf), (lt >> 1) & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
             if (!ok) break;
             tc_fence_after();
             const uint32_t tacc = tmem + lane_addr + buf * BN;
-            float as = 0.f;  // 8-bit operands: this row's scale
-            if constexpr (kInt8) as = m0 + row < p.m ? __ldg(p.a_scale + m0 + row) : 0.f;
+            // the staged scale and bias of tile column c: cscale + 4 c, cbias + 2 c
+            const uint32_t cscale = sbase + S::col, cbias = cscale + 4u * BN;
             if constexpr (kEpi == kAccum) {
                 // fp32 boxes of 32 columns, added into the residual by TMA
 #pragma unroll 1
@@ -424,21 +458,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int c = c_begin + 32 * q;
                     uint32_t acc[32];
                     uint4 braw[4];
-                    float4 ws[8];
                     tmem_ld32(tacc + c, acc);
-                    if constexpr (kInt8) {
-                        fetch_bias_n<T>(bias, n0 + c, p.n, braw);
-                        fetch_scale<32>(p.w_scale, n0 + c, p.n, ws);
-                    } else {
-                        fetch_bias32<T>(bias, n0 + c, braw);
-                    }
+                    if constexpr (!kInt8) fetch_bias32<T>(bias, n0 + c, braw);
                     tmem_wait_ld();
                     if (q + 1 == kWarpCols / 32) acc_empty(buf);  // accumulator read out
                     uint32_t w[32];
+                    if constexpr (kInt8) {
 #pragma unroll
-                    for (int d = 0; d < 32; ++d)
-                        w[d] = __float_as_uint((kInt8 ? scaled<32>(acc[d], ws, d, as) : __uint_as_float(acc[d])) +
-                                               bias_at<T>(braw, d));
+                        for (int d = 0; d < 32; d += 4) {
+                            float y[4];
+                            scale4<T>(y, acc + d, as, cscale + 4u * (c + d), cbias + 2u * (c + d));
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[d + e] = __float_as_uint(y[e]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < 32; ++d) w[d] = __float_as_uint(__uint_as_float(acc[d]) + bias_at<T>(braw, d));
+                    }
                     stage_row(srow, lane, w);
                     if (lane == 0 && live && (!kInt8 || n0 + c < p.n)) {
                         tma_reduce_add_2d(&map_out, stg, n0 + c, y0);
@@ -490,29 +526,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int d0 = 0; d0 < 32; d0 += 16) {  // pairs (d, d + 32), 16 at a time
                         uint32_t lo[16], hi[16];
                         uint4 bl[2], bh[2];
-                        float4 wl[4], wh[4];
-                        const bool in_n = !kInt8 || n0 + c < p.n;  // whole heads: n is a multiple of 64
                         tmem_ld16(tacc + c + d0, lo);
                         tmem_ld16(tacc + c + 32 + d0, hi);
+                        if constexpr (!kInt8) {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            bl[q] = bias != nullptr && in_n ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + d0) + q)
+                            bl[q] = bias != nullptr ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + d0) + q)
                                                     : make_uint4(0, 0, 0, 0);
-                            bh[q] = bias != nullptr && in_n
+                            bh[q] = bias != nullptr
                                         ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + 32 + d0) + q)
                                         : make_uint4(0, 0, 0, 0);
                         }
-                        if constexpr (kInt8) {
-                            fetch_scale<16>(p.w_scale, n0 + c + d0, p.n, wl);
-                            fetch_scale<16>(p.w_scale, n0 + c + 32 + d0, p.n, wh);
                         }
                         tmem_wait_ld();
                         float a[16], b[16];
                         if constexpr (kInt8) {  // rounded once, after the rotation
 #pragma unroll
-                            for (int d = 0; d < 16; ++d) {
-                                a[d] = scaled<16>(lo[d], wl, d, as) + to_f<T>(reinterpret_cast<const T*>(bl)[d]);
-                                b[d] = scaled<16>(hi[d], wh, d, as) + to_f<T>(reinterpret_cast<const T*>(bh)[d]);
+                            for (int d = 0; d < 16; d += 4) {
+                                const int at = c + d0 + d;
+                                scale4<T>(a + d, lo + d, as, cscale + 4u * at, cbias + 2u * at);
+                                scale4<T>(b + d, hi + d, as, cscale + 4u * at + 128, cbias + 2u * at + 64);
                             }
                         } else
 #pragma unroll
@@ -560,10 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint4 b0[4], b1[4];
                     tmem_ld32(tacc + c, a0);
                     tmem_ld32(tacc + c + 32, a1);
-                    if constexpr (kInt8) {
-                        fetch_bias_n<T>(bias, n0 + c, p.n, b0);
-                        fetch_bias_n<T>(bias, n0 + c + 32, p.n, b1);
-                    } else {
+                    if constexpr (!kInt8) {
                         fetch_bias32<T>(bias, n0 + c, b0);
                         fetch_bias32<T>(bias, n0 + c + 32, b1);
                     }
@@ -571,26 +601,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (c + 64 == c_begin + kWarpCols) acc_empty(buf);
                     uint32_t w[32];
                     if constexpr (kInt8) {
-                        float4 ws[8];
-                        fetch_scale<32>(p.w_scale, n0 + c, p.n, ws);
 #pragma unroll
-                        for (int q = 0; q < 16; ++q)
-                            w[q] = DTypeTraits<T>::pack(scaled<32>(a0[2 * q], ws, 2 * q, as) + bias_at<T>(b0, 2 * q),
-                                                        scaled<32>(a0[2 * q + 1], ws, 2 * q + 1, as) +
-                                                            bias_at<T>(b0, 2 * q + 1));
-                        fetch_scale<32>(p.w_scale, n0 + c + 32, p.n, ws);
+                        for (int q = 0; q < 8; ++q) {
+                            float y[4];
+                            const int at = c + 4 * q;
+                            scale4<T>(y, a0 + 4 * q, as, cscale + 4u * at, cbias + 2u * at);
+                            w[2 * q] = DTypeTraits<T>::pack(y[0], y[1]);
+                            w[2 * q + 1] = DTypeTraits<T>::pack(y[2], y[3]);
+                            scale4<T>(y, a1 + 4 * q, as, cscale + 4u * at + 128, cbias + 2u * at + 64);
+                            w[16 + 2 * q] = DTypeTraits<T>::pack(y[0], y[1]);
+                            w[16 + 2 * q + 1] = DTypeTraits<T>::pack(y[2], y[3]);
+                        }
+                    } else {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q)
-                            w[16 + q] = DTypeTraits<T>::pack(
-                                scaled<32>(a1[2 * q], ws, 2 * q, as) + bias_at<T>(b1, 2 * q),
-                                scaled<32>(a1[2 * q + 1], ws, 2 * q + 1, as) + bias_at<T>(b1, 2 * q + 1));
-                    } else
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        w[q] = DTypeTraits<T>::pack(__uint_as_float(a0[2 * q]) + bias_at<T>(b0, 2 * q),
-                                                    __uint_as_float(a0[2 * q + 1]) + bias_at<T>(b0, 2 * q + 1));
-                        w[16 + q] = DTypeTraits<T>::pack(__uint_as_float(a1[2 * q]) + bias_at<T>(b1, 2 * q),
-                                                         __uint_as_float(a1[2 * q + 1]) + bias_at<T>(b1, 2 * q + 1));
+                        for (int q = 0; q < 16; ++q) {
+                            w[q] = DTypeTraits<T>::pack(__uint_as_float(a0[2 * q]) + bias_at<T>(b0, 2 * q),
+                                                        __uint_as_float(a0[2 * q + 1]) + bias_at<T>(b0, 2 * q + 1));
+                            w[16 + q] = DTypeTraits<T>::pack(__uint_as_float(a1[2 * q]) + bias_at<T>(b1, 2 * q),
+                                                             __uint_as_float(a1[2 * q + 1]) + bias_at<T>(b1, 2 * q + 1));
+                        }
                     }
                     stage_row(srow, lane, w);
                     if (lane == 0 && live && (!kInt8 || n0 + c < p.n)) {
@@ -599,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+            if constexpr (kInt8) warp_arrive(bar(S::kColEmpty), lane);
         }
         // the copies out of the staging boxes have landed before the CTA exits
         if (lane == 0) bulk_wait_all();
