@@ -181,14 +181,68 @@ __device__ __forceinline__ void reduce(float (&v)[R], float* red, Op op) {
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r) v[r] = Op::zero();
-    for (int w = 0; w < warps; ++w) {
-        if constexpr (R == 4) {
-            const float4 t = *reinterpret_cast<const float4*>(red + 4 * w);
-            v[0] = op(v[0], t.x), v[1] = op(v[1], t.y), v[2] = op(v[2], t.z), v[3] = op(v[3], t.w);
-        } else {
-            v[0] = op(v[0], red[w]);
+    if (warps <= 4) {
+        for (int w = 0; w < warps; ++w) {
+            if constexpr (R == 4) {
+                const float4 t = *reinterpret_cast<const float4*>(red + 4 * w);
+                v[0] = op(v[0], t.x), v[1] = op(v[1], t.y), v[2] = op(v[2], t.z), v[3] = op(v[3], t.w);
+            } else {
+                v[0] = op(v[0], red[w]);
+            }
         }
+    } else if constexpr (R == 4) {
+        // many warps: two lanes take a warp's four rows, two rows each
+        float2 t = (lane >> 1) < warps ? *reinterpret_cast<const float2*>(red + 2 * lane) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int d = 2; d < 32; d <<= 1) {
+            t.x = op(t.x, __shfl_xor_sync(0xffffffffu, t.x, d));
+            t.y = op(t.y, __shfl_xor_sync(0xffffffffu, t.y, d));
+        }
+        const float ox = __shfl_xor_sync(0xffffffffu, t.x, 1), oy = __shfl_xor_sync(0xffffffffu, t.y, 1);
+        const bool upper = (lane & 1) != 0;
+        v[0] = upper ? ox : t.x, v[1] = upper ? oy : t.y, v[2] = upper ? t.x : ox, v[3] = upper ? t.y : oy;
+    } else {
+        float t = (lane & 15) < warps ? red[lane & 15] : 0.f;
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) t = op(t, __shfl_xor_sync(0xffffffffu, t, d));
+        v[0] = t;
     }
+}
+
+// The largest magnitude of 8 values (packed pairs; a NaN anywhere gives NaN).
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& r);
+template <>
+__device__ __forceinline__ float largest<__half>(const uint4& r) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+}
+template <>
+__device__ __forceinline__ float largest<__nv_bfloat16>(const uint4& r) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+}
+
+// The scale of a quantised row with largest magnitude `big`, and the factor of
+// its values: a row with an infinity or a NaN gets the scale NaN (its products say
+// so), one whose 127 / max could overflow is zero.
+__device__ __forceinline__ float row_scale(float big, float& inv) {
+    const bool finite = __float_as_uint(big) < 0x7f800000u, tiny = big < 7.888609e-31f;  // 2^-100
+    inv = finite && !tiny ? __fdiv_rn(127.f, big) : 0.f;
+    return finite ? (tiny ? 0.f : __fdiv_rn(big, 127.f)) : __uint_as_float(0x7fffffffu);
+}
+
+// rint(v * inv) of 8 values as bytes, from the 1.5 * 2^23 shifter: the low byte of
+// the sum's bits is the integer (|v * inv| <= 127; the product is rounded first, as
+// a separate multiply and rint would).
+__device__ __forceinline__ uint2 quantise8(const float (&v)[8], float inv) {
+    uint32_t u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e], inv), 12582912.f));
+    return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
 }
 
 // t <- LayerNorm / RMS norm of its rows without the vectors (columns past c hold
@@ -393,6 +447,44 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kMode == kQuantOnly && NCH == 
                 unpack8<T>(a, v);
             }
         };
+        if constexpr (kMode == kQuantOnly) {
+            // the values stay packed until they are written
+            uint4 raw[R][NCH];
+            float big[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                big[r] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const bool on = in[i] && r < this_n;
+                    raw[r][i] = on ? ld_shared_u4(chunk((slot + r) & (Rg::kRows - 1), i) + 16u * threadIdx.x) : make_uint4(0, 0, 0, 0);
+                    big[r] = MaxBits{}(big[r], largest<T>(raw[r][i]));
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (r < this_n) fetch();
+            reduce<R>(big, red_all + (parity * kSlots + 4) * kMaxWarps * R, MaxBits{});
+            parity ^= 1;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r >= this_n) continue;
+                float inv;
+                const float scale = row_scale(big[r], inv);
+                if (threadIdx.x == 0) p.h_scale[this_row + r] = scale;
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    if (!in[i]) continue;
+                    float v[8];
+                    unpack8<T>(raw[r][i], v);
+                    *reinterpret_cast<uint2*>(oh + r * oh_step + static_cast<int64_t>(8 * i) * blockDim.x) = quantise8(v, inv);
+                }
+            }
+            oh += this_n * oh_step;
+            this_row += this_n;
+            continue;
+        }
         float x[R][NCH][8];
         float* red = red_all + parity * kSlots * kMaxWarps * R;
         parity ^= 1;
@@ -467,13 +559,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kMode == kQuantOnly && NCH == 
                 if (r >= this_n) continue;
                 float inv = 0.f;
                 if constexpr (kQuant) {
-                    // a row with an infinity or a NaN gets the scale NaN (its products
-                    // say so); one whose 127 / max could overflow is zero
-                    const bool finite = __float_as_uint(big[r]) < 0x7f800000u, tiny = big[r] < 7.888609e-31f;  // 2^-100
-                    inv = finite && !tiny ? __fdiv_rn(127.f, big[r]) : 0.f;
-                    if (threadIdx.x == 0)
-                        p.h_scale[this_row + r] =
-                            finite ? (tiny ? 0.f : __fdiv_rn(big[r], 127.f)) : __uint_as_float(0x7fffffffu);
+                    const float scale = row_scale(big[r], inv);
+                    if (threadIdx.x == 0) p.h_scale[this_row + r] = scale;
                 }
 #pragma unroll
                 for (int i = 0; i < NCH; ++i) {
@@ -481,17 +568,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kMode == kQuantOnly && NCH == 
                     const float(&v)[8] = x[r][i];
                     char* to = oh + r * oh_step + static_cast<int64_t>(8 * i) * blockDim.x * (kQuant ? 1 : 2);
                     if constexpr (kQuant) {
-                        // rint(h * inv) from the 1.5 * 2^23 shifter: the low byte of the
-                        // sum's bits is the integer (|h * inv| <= 127; the product is
-                        // rounded first, as a separate multiply and rint would)
-                        uint32_t u[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(__fadd_rn(__fmul_rn(v[e], inv), 12582912.f));
-                        const uint32_t lo =
-                            __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-                        const uint32_t hi =
-                            __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
-                        *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+                        *reinterpret_cast<uint2*>(to) = quantise8(v, inv);
                     } else {
                         *reinterpret_cast<uint4*>(to) = make_uint4(
                             pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
