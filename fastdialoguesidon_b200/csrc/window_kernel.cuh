@@ -110,7 +110,8 @@ struct TileSmem {
     static constexpr int q = 0;
     static constexpr int k = q + kTileBytes;
     static constexpr int v = k + kKStages * kTileBytes;
-    static constexpr int bars = v + kVStages * kTileBytes;
+    static constexpr int stage = v + kVStages * kTileBytes;  // 2 KB per softmax warp: 64-byte halves of its output rows
+    static constexpr int bars = stage + 4 * 2048;
     static constexpr int kQ = 0;
     static constexpr int kKFull = 1;
     static constexpr int kVFull = kKFull + kKStages;
@@ -253,6 +254,44 @@ inline __device__ __noinline__ void zero_unseen(uint32_t rec, int x0, uint32_t t
     __syncwarp();
 }
 
+// The 32 output rows of a warp (row `lane` of it in this thread, scaled by inv) of
+// the unit {b, h, row0, n}: in two halves through shared memory, so that four lanes
+// write 64 contiguous bytes of a row (a row per lane would write 16 bytes of 32
+// rows' sectors at a time). 16-byte piece c of row r is staged at c ^ (r / 2 & 3).
+template <typename T>
+__device__ __forceinline__ void store_rows(uint32_t stage, const Params& p, int4 at, int first_row, int lane,
+                                           const float (&o)[64], float inv) {
+    T* base = static_cast<T*>(p.out) + at.x * p.out_stride[0];
+    T* to[4];  // of the rows this lane writes pieces of, or null
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int row = first_row + 8 * k + (lane >> 2), query = row / p.pack;
+        to[k] = query < at.w ? base + (at.z + query) * p.out_stride[1] + (at.y + row - query * p.pack) * p.out_stride[2] + 8 * (lane & 3)
+                             : nullptr;
+    }
+    const uint32_t mine = stage + 64u * lane;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        __syncwarp();  // the previous half (or unit) is read out
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float* v = o + 32 * half + 8 * c;
+            st_shared_v4(mine + 16u * (c ^ ((lane >> 1) & 3)),
+                         make_int4(static_cast<int>(DTypeTraits<T>::pack(v[0] * inv, v[1] * inv)),
+                                   static_cast<int>(DTypeTraits<T>::pack(v[2] * inv, v[3] * inv)),
+                                   static_cast<int>(DTypeTraits<T>::pack(v[4] * inv, v[5] * inv)),
+                                   static_cast<int>(DTypeTraits<T>::pack(v[6] * inv, v[7] * inv))));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = 8 * k + (lane >> 2);
+            const int4 v = ld_shared_v4(stage + 64u * r + 16u * ((lane & 3) ^ ((r >> 1) & 3)));
+            if (to[k] != nullptr) *reinterpret_cast<int4*>(to[k] + 32 * half) = v;
+        }
+    }
+}
+
 // The grid has a CTA (or cluster) per unit; a CTA that finishes early takes over
 // the units of CTAs that have not started, so that the next unit's copies and
 // first scores run under the present one's last tiles and epilogue.
@@ -324,7 +363,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
     if (warp >= 4) {
         setmaxnreg_inc<kSoftmaxRegs>();
         const int row = ((warp & 3) << 5) + lane;
-        const int query = row / p.pack, head = row - query * p.pack;  // of this row in its unit
+        const int query = row / p.pack;  // of this row in its unit
         const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
         RowSoftmax<T, false> rs;
         rs.tS = tmem + lane_addr;
@@ -385,10 +424,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
             }
             if (split == 1) {
                 const int4 at = ld_shared_v4(record(i));  // b, h, row0, n: not held in registers over the tiles
-                if (ok && query < at.w)
-                    store_row<T>(static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + query) * p.out_stride[1] +
-                                     (at.y + head) * p.out_stride[2],
-                                 o, none ? 1.f : 1.f / rs.l_run);
+                if (ok)
+                    store_rows<T>(sbase + S::stage + 2048u * (warp & 3), p, at, (warp & 3) * 32, lane, o,
+                                  none ? 1.f : 1.f / rs.l_run);
             } else {
                 const uint32_t part = sbase + S::part + 4u * row;
 #pragma unroll
