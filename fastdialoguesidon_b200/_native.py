@@ -249,6 +249,7 @@ class FdsWindowArgs(ctypes.Structure):
         ("sinks", ctypes.c_int32),
         ("scale", ctypes.c_float),
         ("timeout_ns", ctypes.c_int64),
+        ("debug_flags", ctypes.c_int32),
     ]
 
 

@@ -172,7 +172,7 @@ extern "C" int fds_window_attn_fwd(const FdsWindowArgs* a, void* stream) {
     Params p{};
     p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out;
     p.q_start = a->q_start, p.kv_len = a->kv_len;
-    p.status = a->status, p.status_host = a->status_host, p.timeout_ns = a->timeout_ns;
+    p.status = a->status, p.status_host = a->status_host, p.timeout_ns = a->timeout_ns, p.debug_flags = a->debug_flags;
     for (int i = 0; i < 3; ++i) {
         p.q_stride[i] = a->q_stride[i], p.k_stride[i] = a->k_stride[i];
         p.v_stride[i] = a->v_stride[i], p.out_stride[i] = a->out_stride[i];

@@ -435,14 +435,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 warp_arrive(bar(S::kAccEmpty + b), lane);
             }
         };
+        // 8-bit operands: this row's scale in tile t, fetched a tile ahead
+        const auto row_scale = [&](int t) {
+            const int m = t < p.tiles ? (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM + row : p.m;
+            return m < p.m ? __ldg(p.a_scale + m) : 0.f;
+        };
+        float as_next = 0.f;
+        if constexpr (kInt8) as_next = row_scale(unit0);
         for (int t = unit0; ok && t < p.tiles; t += units, ++lt) {
             const int buf = lt & 1;
             const int m0 = (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM, n0 = (t % p.tiles_n) * BN;
             const int y0 = m0 + wq * 32;     // the warp's first row; rows >= m are clipped by TMA
             const bool live = y0 < p.m;      // a box wholly past the last row is not copied
-            float as = 0.f;  // 8-bit operands: this row's scale
+            const float as = as_next;  // 8-bit operands: this row's scale
             if constexpr (kInt8) {
-                as = m0 + row < p.m ? __ldg(p.a_scale + m0 + row) : 0.f;
+                as_next = row_scale(t + units);
                 ok = warp_wait(bar(S::kColFull), lt & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
             }
             if (ok) ok = warp_wait(bar(S::kAccFull + buf), (lt >> 1) & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);

@@ -211,7 +211,7 @@ void batch_vector(const Tensor* t, const char* name, c10::Device dev, int64_t ba
     vector_1d(*t, name, batch, 4);
 }
 
-// (q, k, v, left, right, sinks, q_start, kv_len, out, scale, timeout_ns)
+// (q, k, v, left, right, sinks, q_start, kv_len, out, scale, timeout_ns, debug_flags)
 PyObject* window_attention(PyObject* const* a) {
     const Tensor& q = required(a[0], "q");
     type_is16(q, "q");
@@ -265,6 +265,7 @@ PyObject* window_attention(PyObject* const* a) {
         w.sinks = static_cast<int32_t>(std::min(sinks, top));
         w.scale = static_cast<float>(scale);
         w.timeout_ns = integer(a[10], "timeout_ns");
+        w.debug_flags = static_cast<int32_t>(integer(a[11], "debug_flags"));
         launch(g_window, w, dev, "fds_window_attn_fwd");
     }
     return THPVariable_Wrap(out);
@@ -562,7 +563,7 @@ PyMethodDef method(const char* name) {
 
 PyMethodDef g_methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
-    method<window_attention, 11>("window_attention"),
+    method<window_attention, 12>("window_attention"),
     method<quantize_rows, 3>("quantize_rows"),
     method<linear_int8, 14>("linear_int8"),
     method<residual_norm, 19>("residual_norm"),

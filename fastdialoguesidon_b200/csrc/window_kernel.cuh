@@ -58,6 +58,7 @@ struct Params {
     int32_t* status_host;
     int64_t timeout_ns;
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];  // elements: batch, row, head
+    int32_t debug_flags;
     int32_t heads, kv_heads, q_len, k_len;
     int32_t left, right, sinks;
     // tile kernel: `pack` heads of a unit (those of one key head, or 1) and
@@ -127,7 +128,8 @@ struct TileSmem {
     static constexpr int kRecFull = kDrain + 1;     // [record] laid out
     static constexpr int kRecEmpty = kRecFull + 2;  // [record] read by every role
     static constexpr int kNext = kRecEmpty + 2;     // the next unit's launch-control answer landed
-    static constexpr int kNumBars = kNext + 1;
+    static constexpr int kNever = kNext + 1;
+    static constexpr int kNumBars = kNever + 1;
     static constexpr int misc = bars + kNumBars * 8;  // the bounded waits' block (attn_kernel.cuh Smem::misc)
     static constexpr int records = (misc + 48 + 15) / 16 * 16;
     static constexpr int answer = records + 2 * 64;
@@ -325,6 +327,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
             mbar_init(&bars[S::kRecEmpty + r], kRecordReaders);
         }
         mbar_init(&bars[S::kNext], 1);
+        mbar_init(&bars[S::kNever], 1);
         st_shared_volatile_u32(ctl.misc + 4, 0);
         st_shared_u64(ctl.misc + 8, reinterpret_cast<uint64_t>(p.status));
         st_shared_u64(ctl.misc + 16, static_cast<uint64_t>(p.timeout_ns > 0 ? p.timeout_ns : kDefaultTimeoutNs));
@@ -461,6 +464,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
             constexpr int err = FDS_STATUS_TIMEOUT_MMA;
             int g = 0, q = 0;  // tiles and units so far (ring stages and barrier phases run on)
             bool ok = true;
+            // test hook: a wait on a barrier that nothing arrives on, to exercise the
+            // bounded-wait error path without a real hang
+            if (p.debug_flags & FDS_DEBUG_FORCE_TIMEOUT) ok = warp_wait(bar(S::kNever), 0, ctl, err);
             // S columns <- Q K(tile g)^T, once the previous scores are read out; the unit's last also frees Q
             const auto scores = [&](int gt, bool last) {
                 if (gt > 0) ok = warp_wait(bar(S::kSFree), (gt - 1) & 1, ctl, err);

@@ -64,7 +64,8 @@ def _load():
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: int, right: int = 0, sinks: int = 0,
                      q_start: torch.Tensor | None = None, kv_len: torch.Tensor | None = None,
-                     out: torch.Tensor | None = None, *, scale: float | None = None, timeout_ns: int = 0) -> torch.Tensor:
+                     out: torch.Tensor | None = None, *, scale: float | None = None, timeout_ns: int = 0,
+                     debug_flags: int = 0) -> torch.Tensor:
     """Softmax attention of each query over a window of keys and the first ``sinks`` keys.
 
     q [B, Lq, H, 64], k and v [B, Lk, Hk, 64] fp16 / bf16, H a multiple of Hk
@@ -84,7 +85,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     A stream's next frame: ``q`` with Lq = 1, its cache as k and v with the
     frame's own key and value written at ``q_start``, ``right=0``.
     """
-    return (_ext or _load()).window_attention(q, k, v, left, right, sinks, q_start, kv_len, out, scale, timeout_ns)
+    return (_ext or _load()).window_attention(q, k, v, left, right, sinks, q_start, kv_len, out, scale, timeout_ns,
+                                              debug_flags)
 
 
 # ---------------------------------------------------------------- 8-bit projections

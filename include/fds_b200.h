@@ -402,6 +402,7 @@ typedef struct FdsWindowArgs {
     int32_t sinks;
     float scale;              /* softmax scale on q . k */
     int64_t timeout_ns;       /* bound on every in-kernel wait; <= 0 selects 2 s */
+    int32_t debug_flags;      /* 0 in production */
 } FdsWindowArgs;
 
 FDS_API int fds_window_attn_fwd(const FdsWindowArgs* args, void* stream);

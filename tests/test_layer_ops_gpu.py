@@ -18,10 +18,14 @@ and v = 2^-24 that of fp32:
 * row quantisation: equal, value for value (its definition is in fp32).
 """
 
+import importlib.util
+from pathlib import Path
+
 import pytest
 import torch
 
 import fastdialoguesidon_b200 as F
+from fastdialoguesidon_b200 import _native as N
 from oracle import layer_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -420,3 +424,88 @@ def test_on_another_stream_and_in_a_graph(cuda_device):
     torch.cuda.synchronize()
     F.check_status()
     assert all(torch.equal(a, c) for a, c in zip(want, held))
+
+
+@pytest.mark.parametrize("frames", [777, 1501])
+def test_example_layer(cuda_device, frames):
+    """The example's layer against fp32. Row and channel quantisation to 8 bits
+    leave each operand of a projection about 42 dB (768 values, largest near 3.2
+    deviations: a step of 2 * 3.2 / 254), two projections with both operands
+    quantised about 36 dB; 30 dB is asked. The stream runs the same kernels but for
+    the order of sums and the weights' rounding point: a few values may round to
+    the neighbouring 8-bit step; 45 dB is asked."""
+    path = Path(__file__).resolve().parents[1] / "examples" / "long_recording_int8.py"
+    spec = importlib.util.spec_from_file_location("long_recording_int8", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    result = example.main(frames)
+    assert result["update_snr_db"] >= 30.0 and result["stream_snr_db"] >= 45.0, result
+
+
+def test_torch_operators(cuda_device):
+    q, k, v = _qkv(1, 200, 200, 2, 2, torch.float16, seed=1)
+    want = F.window_attention(q, k, v, 30, 4, 2)
+    assert torch.equal(torch.ops.fds.window_attention(q, k, v, 30, 4, 2), want)
+    out = torch.empty_like(want)
+    assert torch.ops.fds.window_attention(q, k, v, 30, 4, 2, out=out).data_ptr() == out.data_ptr() and torch.equal(out, want)
+    ops = _cuda(*_int8_operands(30, 64, 128, torch.bfloat16, bias=True, seed=1))
+    assert torch.equal(torch.ops.fds.linear_int8(*ops), F.linear_int8(*ops))
+    with torch.device("meta"):
+        m = torch.empty(1, 9, 2, 64, dtype=torch.float16)
+        assert torch.ops.fds.window_attention(m, m, m, 3).shape == m.shape
+
+
+@pytest.mark.parametrize("Lq,Lk,left", [(300, 300, 50), (40, 3000, 2900)])
+def test_window_bounded_wait(cuda_device, Lq, Lk, left):
+    """A wait that runs out reports itself, in whole units and in a split one, and
+    the next call (after the status is cleared) is right."""
+    q, k, v = _qkv(1, Lq, Lk, 2, 2, torch.float16, seed=1)
+    start = _i32(Lk - Lq)
+    F.window_attention(q, k, v, left, 0, 2, q_start=start, timeout_ns=2_000_000, debug_flags=N.FDS_DEBUG_FORCE_TIMEOUT)
+    with pytest.raises(F.FdsError, match="timeout"):
+        F.check_status()
+    _check_window(q[:, :40], k, v, left, 0, 2, q_start=start)
+
+
+def test_residual_norm_rows_on_16_byte_boundaries(cuda_device):
+    """fp32 rows that are 16- but not 32-byte aligned (no 256-bit accesses)."""
+    g = _gen(21)
+    wide = torch.randn(50, 520, generator=g).cuda()
+    x, y = wide[:, 4:516], torch.randn(50, 512, generator=g).half().cuda()
+    keep = torch.zeros(50, 520, device="cuda")[:, 4:516]
+    rx, rh = O.residual_norm(x.cpu(), y.cpu())
+    x1, h = F.residual_norm(x, y, residual_out=keep)
+    assert bool(((x1.cpu().double() - rx).abs() <= V * rx.abs()).all())
+    assert bool(((h.cpu().double() - rh).abs() <= U[torch.float16] * rh.abs() + 2.0 ** -17 * rh.abs().amax(1, keepdim=True)).all())
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Caches and matrices of more than 2^31 elements: the rows that matter lie past that."""
+    Lk, Hk = 1_060_000, 32  # 2.2e9 elements
+    k = torch.empty(1, Lk, Hk, 64, dtype=torch.float16, device="cuda")
+    v = torch.empty(1, Lk, Hk, 64, dtype=torch.float16, device="cuda")
+    g = _gen(31)
+    tail = torch.randn(2, 1, 700, Hk, 64, generator=g).half()
+    k[:, -700:], v[:, -700:] = tail[0].cuda(), tail[1].cuda()
+    for Lq in (1, 70):
+        q = torch.randn(1, Lq, Hk, 64, generator=g).half().cuda()
+        got = F.window_attention(q, k, v, 500, 0, 0, q_start=_i32(Lk - Lq))
+        ref = O.window_attention(q.cpu(), tail[0], tail[1], 500, 0, 0, [700 - Lq])
+        assert float((got.cpu().double() - ref).abs().max()) <= (2 * U[torch.float16] + 2e-4) * float(tail[1].abs().max())
+    del k, v
+    m, kk, n = 530_000, 4096, 16  # 2.2e9 elements
+    x = torch.ones(m, kk, dtype=torch.float16, device="cuda")
+    x[-40:] = torch.randn(40, kk, generator=g).half().cuda()
+    w, ws = torch.randint(-127, 128, (n, kk), generator=g, dtype=torch.int8), torch.rand(n, generator=g) * 1e-2
+    xq, xs = F.quantize_rows(x)
+    qr, sr = O.quantize_rows(x[-40:].cpu())
+    assert torch.equal(xq[-40:].cpu(), qr) and torch.equal(xs[-40:].cpu(), sr)
+    got = F.linear_int8(xq, xs, w.cuda(), ws.cuda())
+    prod, ref = O.linear_int8(qr, sr, w, ws)
+    _check_linear(got[-40:], prod, ref, torch.float16)
+    F.check_status()
+    h = torch.empty_like(x)
+    _, out = F.residual_norm(x, out=h)
+    _, rh = O.residual_norm(x[-40:].cpu())
+    err = (out[-40:].cpu().double() - rh).abs()
+    assert bool((err <= U[torch.float16] * rh.abs() + 2.0 ** -17 * rh.abs().amax(1, keepdim=True)).all())
