@@ -554,7 +554,8 @@ def linear_rope(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, cos: t
     _check(length >= 1, "length must be >= 1")
     _rope_tables(cos, sin, min(length, x.shape[0]), x)
     out = _linear_out(x, n, out, x.dtype)
-    return _linear_call(x, w, b, out, N.FDS_EPILOGUE_ROPE, cos=cos, sin=sin, seq_len=length,
+    # (the table has min(length, rows) rows at least: positions past the last row do not occur)
+    return _linear_call(x, w, b, out, N.FDS_EPILOGUE_ROPE, cos=cos, sin=sin, seq_len=min(length, max(1, x.shape[0])),
                         rope_cols=2 * heads * HEAD_DIM, grid_ctas=grid_ctas, pair=pair)
 
 
