@@ -26,20 +26,45 @@ int launch(Params& p, int threads, int per_sm, int sms, cudaStream_t stream) {
 }
 
 // A CTA as wide as the row: 8 columns a thread up to 4096, 16 or 32 beyond. The
-// grid is what the SMs hold at once (16 warps each at 128 registers, 32 for the
-// quantiser at 64); four rows at a time once a CTA has two or more (3000 x 768
+// grid is what the SMs hold at once (16 warps each at 128 registers); four rows at a time once a CTA has two or more (3000 x 768
 // fp32 stream: 6.9 us against 8.3 us row by row, 6000 x 768: 13.9 against 16.9),
 // single rows below, which are bound by one row's latency.
 template <typename T, int kMode, bool kXf32, bool kQuant>
 int launch_shape(Params& p, int sms, cudaStream_t s) {
     const int nch = p.c <= 4096 ? 1 : (p.c <= 8192 ? 2 : 4);
     const int warps = (p.c + 256 * nch - 1) / (256 * nch);
-    const int per_sm = std::max(1, (kMode == kQuantOnly && nch == 1 ? 32 : 16) / warps);
+    const int per_sm = std::max(1, 16 / warps);
     if (nch == 4) return launch<T, 4, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
     if (nch == 2) return launch<T, 2, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
     if (p.rows >= 2 * sms * per_sm) return launch<T, 1, 4, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
     return launch<T, 1, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
 }
+
+template <typename T, int NCH, int kR>
+int launch_quantise(const Params& p, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>((p.rows - 1) / (kQuantWarps * kR) + 1)), block(32 * kQuantWarps);
+    cudaError_t e = launch_pdl(quantise_rows_kernel<T, NCH, kR>, grid, block, 0, stream, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "row quantiser launch: %s", cudaGetErrorString(e));
+    return FDS_OK;
+}
+
+// By the row's width: the chunks a lane holds, and four or two rows a warp where
+// one row would leave it less than 1 KB in flight.
+template <typename T>
+int launch_quantise_width(const Params& p, cudaStream_t s) {
+    const int chunks = (p.c + 255) / 256;
+    if (chunks <= 1) return launch_quantise<T, 1, 4>(p, s);
+    if (chunks <= 2) return launch_quantise<T, 2, 2>(p, s);
+    if (chunks <= 3) return launch_quantise<T, 3, 1>(p, s);
+    if (chunks <= 4) return launch_quantise<T, 4, 1>(p, s);
+    if (chunks <= 6) return launch_quantise<T, 6, 1>(p, s);
+    if (chunks <= 8) return launch_quantise<T, 8, 1>(p, s);
+    if (chunks <= 12) return launch_quantise<T, 12, 1>(p, s);
+    if (chunks <= 16) return launch_quantise<T, 16, 1>(p, s);
+    return launch_quantise<T, 32, 1>(p, s);
+}
+constexpr int kQuantWidth = 8192;  // columns a warp's registers hold; wider rows take the norm's kernel
 
 template <typename T, bool kXf32>
 int launch_mode(Params& p, int sms, cudaStream_t s) {
@@ -47,7 +72,7 @@ int launch_mode(Params& p, int sms, cudaStream_t s) {
     if (p.y != nullptr)
         return quant ? launch_shape<T, kBoth, kXf32, true>(p, sms, s) : launch_shape<T, kBoth, kXf32, false>(p, sms, s);
     const bool plain = p.norm == kNone && p.w == nullptr && p.b == nullptr && p.scale == nullptr && p.shift == nullptr;
-    if (quant && plain && !kXf32) return launch_shape<T, kQuantOnly, false, true>(p, sms, s);
+    if (quant && plain && !kXf32 && p.c <= kQuantWidth) return launch_quantise_width<T>(p, s);
     return quant ? launch_shape<T, kNormOnly, kXf32, true>(p, sms, s) : launch_shape<T, kNormOnly, kXf32, false>(p, sms, s);
 }
 
