@@ -357,6 +357,34 @@ def test_residual_norm(cuda_device, rows, c, post, norm, gate, mod, windows, dty
     assert x2.data_ptr() == dev["x"].data_ptr() and torch.equal(x2, x1) and torch.equal(h2, h)
 
 
+MANY_ROWS = [
+    (700, 8, "none", "layer", "none", True, 1), (601, 256, "rms", "rms", "layer", False, 3), (1203, 264, "layer", "layer", "window", True, 4),
+    (900, 512, "rms", "layer", "window", True, 2), (777, 768, "layer", "rms", "layer", True, 7), (650, 776, "none", "layer", "window", True, 2),
+    (1300, 1024, "layer", "none", "none", True, 5), (611, 1032, "rms", "layer", "window", True, 2)]
+
+
+@pytest.mark.parametrize("rows,c,post,norm,gate,mod,windows", MANY_ROWS)
+@pytest.mark.parametrize("dtype,stream,pdtype", [(torch.float16, torch.float32, torch.float16), (torch.bfloat16, torch.bfloat16, torch.bfloat16),
+                                                 (torch.bfloat16, torch.float32, torch.float32), (torch.float16, torch.float16, torch.float32)])
+def test_residual_norm_many_rows(cuda_device, rows, c, post, norm, gate, mod, windows, dtype, stream, pdtype):
+    """As test_residual_norm, for more rows than four to an SM."""
+    test_residual_norm(cuda_device, rows, c, post, norm, gate, mod, windows, dtype, stream, pdtype)
+
+
+@pytest.mark.parametrize("c", [512, 1024])
+def test_residual_norm_many_rows_without_a_block(cuda_device, c):
+    """The norm alone, on column slices whose rows are 16- but not 32-byte aligned; what lies beside them stays."""
+    g = _gen(c)
+    x = torch.randn(1500, c + 8, generator=g).cuda()[:, 4:c + 4]
+    out = torch.zeros(1500, c + 16, dtype=torch.bfloat16, device="cuda")
+    scale, shift = torch.randn(c, generator=g).cuda(), torch.randn(c, generator=g).cuda()
+    _, rh = O.residual_norm(x.cpu(), None, scale=scale.cpu(), shift=shift.cpu())
+    _, h = F.residual_norm(x, None, scale=scale, shift=shift, dtype=torch.bfloat16, out=out[:, 8:c + 8])
+    big = rh.abs().amax(1, keepdim=True) + shift.cpu().double().abs().max()
+    assert bool(((h.cpu().double() - rh).abs() <= U[torch.bfloat16] * rh.abs() + 2.0 ** -17 * big).all())
+    assert float(out[:, :8].abs().max()) == 0.0 and float(out[:, c + 8:].abs().max()) == 0.0
+
+
 def test_residual_norm_without_a_block(cuda_device):
     case = _norm_case(41, 768, torch.float16, torch.float32, "none", "layer", "none", True, 2, torch.float16, seed=1)
     case["y"] = None
