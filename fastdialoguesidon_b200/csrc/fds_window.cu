@@ -84,6 +84,11 @@ int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream)
         (rc = make_heads_map(&maps.v8, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, 8)) != FDS_OK)
         return rc;
     p.row_blocks = (p.q_len + p.queries - 1) / p.queries;
+    // a warp's 32 output rows are whole queries: one box each (else a row per thread)
+    p.out_boxes = 32 % p.pack == 0;
+    maps.out = maps.q;
+    if (p.out_boxes && (rc = make_heads_map(&maps.out, a->out, a->dtype, p.heads, p.q_len, a->batch, p.out_stride, 32 / p.pack, p.pack)) != FDS_OK)
+        return rc;
     const int64_t units = static_cast<int64_t>(a->batch) * (p.heads / p.pack) * p.row_blocks;
     // A unit's tiles are dealt to a cluster while that still fills idle SMs
     // (two CTAs each) and leaves every CTA two tiles.

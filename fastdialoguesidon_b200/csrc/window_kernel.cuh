@@ -17,7 +17,7 @@
 //   their own columns and not a tile of their own, and at most one tile at the
 //   left edge and two at the right are seen in part. The step is the
 //   bidirectional attention's (attn_kernel.cuh RowSoftmax). A CTA has one query
-//   tile and half an SM (128 + 128 threads, 256 TMEM columns, 98 KB): a window is
+//   tile and half an SM (128 + 128 threads, 256 TMEM columns, 112 KB): a window is
 //   a handful of tiles, and a 128-row tile overlaps fewer keys that its rows do
 //   not see than a 256-row unit. With few query tiles and many key tiles the
 //   column tiles of a unit are dealt to a cluster of up to 8 CTAs, whose partial
@@ -65,6 +65,7 @@ struct Params {
     // `queries` = 128 / pack of each; row r of a unit is query r / pack, head r % pack
     int32_t pack, queries;
     int32_t row_blocks;  // ceil(q_len / queries)
+    int32_t out_boxes;   // pack divides 32: a warp's output rows are a box of heads x queries
     float scale_log2;
 };
 
@@ -111,8 +112,8 @@ struct TileSmem {
     static constexpr int q = 0;
     static constexpr int k = q + kTileBytes;
     static constexpr int v = k + kKStages * kTileBytes;
-    static constexpr int stage = v + kVStages * kTileBytes;  // 2 KB per softmax warp: 64-byte halves of its output rows
-    static constexpr int bars = stage + 4 * 2048;
+    static constexpr int stage = v + kVStages * kTileBytes;  // 4 KB per softmax warp: its output rows
+    static constexpr int bars = stage + kTileBytes;
     static constexpr int kQ = 0;
     static constexpr int kKFull = 1;
     static constexpr int kVFull = kKFull + kKStages;
@@ -134,7 +135,7 @@ struct TileSmem {
     static constexpr int records = (misc + 48 + 15) / 16 * 16;
     static constexpr int answer = records + 2 * 64;
     static constexpr int total = answer + 16;
-    static constexpr int alloc = total + 1024;
+    static constexpr int alloc = total;
     // a split unit's partial rows, [66][128] floats (64 of O, max, sum), over the K ring
     static constexpr int part = k;
     static_assert(66 * 128 * 4 <= kKStages * kTileBytes, "partial rows");
@@ -146,6 +147,7 @@ constexpr int kTP = 128, kTO = 192;
 struct Maps {
     CUtensorMap q, k, v;    // boxes of 128 rows
     CUtensorMap k8, v8;     // boxes of 8 rows (tiles that hold sinks and window keys)
+    CUtensorMap out;        // boxes of 32 rows (out_boxes)
 };
 
 // Merge of row `row` of a split unit, the `part_idx`-th of `split` column ranges, into
@@ -256,41 +258,27 @@ inline __device__ __noinline__ void zero_unseen(uint32_t rec, int x0, uint32_t t
     __syncwarp();
 }
 
-// The 32 output rows of a warp (row `lane` of it in this thread, scaled by inv) of
-// the unit {b, h, row0, n}: in two halves through shared memory, so that four lanes
-// write 64 contiguous bytes of a row (a row per lane would write 16 bytes of 32
-// rows' sectors at a time). 16-byte piece c of row r is staged at c ^ (r / 2 & 3).
-template <typename T>
-__device__ __forceinline__ void store_rows(uint32_t stage, const Params& p, int4 at, int first_row, int lane,
-                                           const float (&o)[64], float inv) {
-    T* base = static_cast<T*>(p.out) + at.x * p.out_stride[0];
-    T* to[4];  // of the rows this lane writes pieces of, or null
+// Thread `lane` of a warp has row `lane` of 32 output rows, 64 values in w. Rows
+// [query0 ..] x [head .. head + pack) of window b as one box, through the warp's
+// 4 KB of shared memory (16-byte piece c of a row at c ^ (row & 7)). An epilogue is
+// one warp's dependent instructions, and takes 1000 cycles this way; 2250 with the
+// addresses of 64-byte pieces worked out per lane (600 s of audio in 16 heads: 221
+// us against 214), and rows written by their own threads in 32-byte stores, as few
+// instructions, cost the steps beside them more (226 us).
+__device__ __forceinline__ void store_box(uint32_t stage, const CUtensorMap* map, int lane, const uint32_t (&w)[32], int head,
+                                          int query0, int b, bool any) {
+    if (lane == 0) bulk_wait_read_all();  // the previous unit's rows are read out
+    __syncwarp();
+    const uint32_t mine = stage + 128u * lane;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int row = first_row + 8 * k + (lane >> 2), query = row / p.pack;
-        to[k] = query < at.w ? base + (at.z + query) * p.out_stride[1] + (at.y + row - query * p.pack) * p.out_stride[2] + 8 * (lane & 3)
-                             : nullptr;
-    }
-    const uint32_t mine = stage + 64u * lane;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        __syncwarp();  // the previous half (or unit) is read out
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float* v = o + 32 * half + 8 * c;
-            st_shared_v4(mine + 16u * (c ^ ((lane >> 1) & 3)),
-                         make_int4(static_cast<int>(DTypeTraits<T>::pack(v[0] * inv, v[1] * inv)),
-                                   static_cast<int>(DTypeTraits<T>::pack(v[2] * inv, v[3] * inv)),
-                                   static_cast<int>(DTypeTraits<T>::pack(v[4] * inv, v[5] * inv)),
-                                   static_cast<int>(DTypeTraits<T>::pack(v[6] * inv, v[7] * inv))));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int r = 8 * k + (lane >> 2);
-            const int4 v = ld_shared_v4(stage + 64u * r + 16u * ((lane & 3) ^ ((r >> 1) & 3)));
-            if (to[k] != nullptr) *reinterpret_cast<int4*>(to[k] + 32 * half) = v;
-        }
+    for (int c = 0; c < 8; ++c)
+        st_shared_v4(mine + 16u * (c ^ (lane & 7)), make_int4(static_cast<int>(w[4 * c]), static_cast<int>(w[4 * c + 1]),
+                                                              static_cast<int>(w[4 * c + 2]), static_cast<int>(w[4 * c + 3])));
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && any) {
+        tma_store_4d(map, stage, 0, head, query0, b);
+        bulk_commit_group();
     }
 }
 
@@ -300,10 +288,8 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const Params& p, int4
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __grid_constant__ Maps maps, const Params p) {
     using S = TileSmem;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw_addr = smem_u32(smem_raw);
-    const uint32_t sbase = (raw_addr + 1023u) & ~1023u;
-    uint8_t* smem = smem_raw + (sbase - raw_addr);
+    extern __shared__ __align__(1024) uint8_t smem[];  // the tiles' swizzle repeats every 1024 bytes
+    const uint32_t sbase = smem_u32(smem);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::bars);
     const WaitCtl ctl{sbase + S::misc};
     const auto bar = [&](int idx) { return sbase + S::bars + 8u * idx; };
@@ -339,6 +325,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
         prefetch_tensormap(&maps.q);
         prefetch_tensormap(&maps.k);
         prefetch_tensormap(&maps.v);
+        if (p.out_boxes) prefetch_tensormap(&maps.out);
     }
     if (warp == 2) {
         tmem_alloc(reinterpret_cast<uint32_t*>(smem + S::misc), kTmemColsTile);
@@ -409,36 +396,52 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
                 ok = rs.template step<false, kMaskWindow>(t, 0.f);
             }
             const bool none = rs.m_run == -INFINITY;  // no key seen
-            float o[64];
+            const float inv = none ? 1.f : 1.f / rs.l_run;
+            uint32_t o[64];
             if (ok && t1 > rs.t_begin) {
                 // (the next unit's first P V overwrites O only after this warpgroup's
                 // next P store, which follows this read in program order)
                 ok = warp_wait(rs.pv_done, rs.pv_parity, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
                 rs.pv_parity ^= 1;
                 tc_fence_after();
-                uint32_t ou[64];
-                tmem_ld64(rs.tO, ou);
+                tmem_ld64(rs.tO, o);
                 tmem_wait_ld();
+                if (__any_sync(0xffffffffu, none)) {
 #pragma unroll
-                for (int e = 0; e < 64; ++e) o[e] = none ? 0.f : __uint_as_float(ou[e]);
+                    for (int e = 0; e < 64; ++e) o[e] = none ? 0 : o[e];
+                }
             } else {
 #pragma unroll
-                for (int e = 0; e < 64; ++e) o[e] = 0.f;
+                for (int e = 0; e < 64; ++e) o[e] = 0;
             }
             if (split == 1) {
                 const int4 at = ld_shared_v4(record(i));  // b, h, row0, n: not held in registers over the tiles
-                if (ok)
-                    store_rows<T>(sbase + S::stage + 2048u * (warp & 3), p, at, (warp & 3) * 32, lane, o,
-                                  none ? 1.f : 1.f / rs.l_run);
+                uint32_t w[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float2 v = fmul2(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), make_float2(inv, inv));
+                    w[e] = DTypeTraits<T>::pack(v.x, v.y);
+                }
+                if (p.out_boxes) {
+                    const int q0 = __shfl_sync(0xffffffffu, query, 0);
+                    store_box(sbase + S::stage + 4096u * (warp & 3), &maps.out, lane, w, at.y, at.z + q0, at.x, ok && q0 < at.w);
+                } else if (ok && query < at.w) {
+                    T* to = static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + query) * p.out_stride[1] +
+                            (at.y + row - query * p.pack) * p.out_stride[2];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(to + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+                }
             } else {
                 const uint32_t part = sbase + S::part + 4u * row;
 #pragma unroll
-                for (int e = 0; e < 64; ++e) st_shared_f32(part + 512u * e, o[e]);
+                for (int e = 0; e < 64; ++e) st_shared_f32(part + 512u * e, __uint_as_float(o[e]));
                 st_shared_f32(part + 512u * 64, rs.m_run);
                 st_shared_f32(part + 512u * 65, none ? 0.f : rs.l_run);
             }
             if (split == 1) record_release(i);
         }
+        if (lane == 0) bulk_wait_all();  // the output boxes are written
         __syncwarp();
         tc_fence_before();
         named_barrier_sync(1, kTileThreads);
