@@ -51,6 +51,10 @@ __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t count) 
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
+__device__ __forceinline__ void named_barrier_arrive(uint32_t id, uint32_t count) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
 // ---------------------------------------------------------------- shared-memory scalars
 // 32-bit shared-window addresses keep these accesses to one register operand.
 
@@ -285,6 +289,10 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// ... in two halves
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // The shared::cluster address of the same shared-memory offset in CTA `rank`.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t rank) {
     uint32_t d;
@@ -298,10 +306,11 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
     return r;
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_v4f32(uint32_t cluster_addr, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
 // Launch control: asks to cancel the launch of a CTA of this grid that has not
@@ -312,20 +321,22 @@ __device__ __forceinline__ void launch_control_ask(uint32_t dst, uint32_t bar) {
                  "r"(bar)
                  : "memory");
 }
-// Whether a CTA was cancelled -- its work is the asker's now -- and its blockIdx.x.
-__device__ __forceinline__ bool launch_control_answer(uint32_t src, int& block_x) {
-    uint32_t got, x;
+// Whether a CTA was cancelled -- its work is the asker's now -- and its blockIdx.
+__device__ __forceinline__ bool launch_control_answer(uint32_t src, int (&block)[3]) {
+    uint32_t got, x, y, z;
     asm volatile(
         "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
-        "ld.shared.b128 r, [%2];\n\t"
+        "ld.shared.b128 r, [%4];\n\t"
         "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t"
-        "mov.u32 %1, 0;\n\t"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
-        : "=r"(got), "=r"(x)
+        "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %2, r;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::z.b32.b128 %3, r;\n\t}"
+        : "=r"(got), "=r"(x), "=r"(y), "=r"(z)
         : "r"(src)
         : "memory");
-    if (got != 0) block_x = static_cast<int>(x);
+    block[0] = static_cast<int>(x), block[1] = static_cast<int>(y), block[2] = static_cast<int>(z);
     return got != 0;
 }
 

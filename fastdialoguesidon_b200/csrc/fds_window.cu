@@ -69,6 +69,20 @@ int64_t most_keys(const Params& p, int rows) {
     return std::min<int64_t>(p.k_len, static_cast<int64_t>(p.left) + p.right + rows + p.sinks);
 }
 
+template <typename T, bool kSplit>
+int launch_units(const fds::window::Maps& maps, const Params& p, int batch, int split, cudaStream_t stream) {
+    auto kern = fds::window::window_tile_kernel<T, kSplit>;
+    constexpr int smem = fds::window::TileSmem<kSplit>::alloc;
+    static std::atomic<uint64_t> smem_set{0};
+    cudaError_t e = set_smem_once(kern, smem, smem_set);
+    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "cudaFuncSetAttribute(window): %s", cudaGetErrorString(e));
+    const dim3 grid(static_cast<unsigned>(p.row_blocks * split), static_cast<unsigned>(p.heads / p.pack), static_cast<unsigned>(batch));
+    e = launch_cluster(kern, grid, fds::window::kTileThreads, smem, split, stream, maps, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "window attention launch: %s", cudaGetErrorString(e));
+    return FDS_OK;
+}
+
 template <typename T>
 int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream) {
     // the heads of a key head share units, so that its keys are read once for them
@@ -95,16 +109,8 @@ int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream)
     const int64_t tiles = (most_keys(p, p.queries) + fds::kBlockN - 1) / fds::kBlockN;
     int split = 1;
     while (split < fds::window::kMaxSplit && units * split * 2 <= 2 * sms && tiles >= 4 * split) split *= 2;
-    if (units * split > 0x7fffffffLL) return set_error(FDS_ERR_INVALID_ARGUMENT, "too many query tiles");
-    auto kern = fds::window::window_tile_kernel<T>;
-    static std::atomic<uint64_t> smem_set{0};
-    cudaError_t e = set_smem_once(kern, fds::window::TileSmem::alloc, smem_set);
-    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "cudaFuncSetAttribute(window): %s", cudaGetErrorString(e));
-    e = launch_cluster(kern, dim3(static_cast<unsigned>(units * split)), fds::window::kTileThreads,
-                       fds::window::TileSmem::alloc, split, stream, maps, p);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "window attention launch: %s", cudaGetErrorString(e));
-    return FDS_OK;
+    if (p.heads / p.pack > 65535) return set_error(FDS_ERR_INVALID_ARGUMENT, "more than 65535 heads");
+    return split > 1 ? launch_units<T, true>(maps, p, a->batch, split, stream) : launch_units<T, false>(maps, p, a->batch, 1, stream);
 }
 
 template <typename T, int kHalves, bool kMulti>

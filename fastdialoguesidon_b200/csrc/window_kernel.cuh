@@ -20,8 +20,9 @@
 //   tile and half an SM (128 + 128 threads, 256 TMEM columns, 112 KB): a window is
 //   a handful of tiles, and a 128-row tile overlaps fewer keys that its rows do
 //   not see than a 256-row unit. With few query tiles and many key tiles the
-//   column tiles of a unit are dealt to a cluster of up to 8 CTAs, whose partial
-//   (O, max, sum) are merged through distributed shared memory in rank order.
+//   column tiles of a unit are dealt to a cluster of up to 8 CTAs: each owns some
+//   of the rows, whose partial (O, max, sum) the others store into its shared
+//   memory, and merges them in rank order.
 // * window_step_kernel: up to 16 query rows per key head (a decoding step):
 //   bound by reading the keys and values once. Each warp streams its share of the
 //   keys through a shared-memory ring of its own and multiplies them with the
@@ -105,14 +106,22 @@ constexpr int kTileThreads = 256;
 constexpr int kTileRegs = 128;  // per thread at launch: 65536 / (2 CTAs x 256)
 constexpr int kSoftmaxRegs = 200, kControlRegs = 56;
 static_assert(128 * kSoftmaxRegs + 128 * kControlRegs <= kTileThreads * kTileRegs, "register split exceeds the launch pool");
-constexpr int kKStages = 3, kVStages = 2;
+constexpr int kVStages = 2;
 constexpr int kMaxSplit = 8;
 
+// kSplit: units dealt to clusters. Such a CTA needs no staged output rows, and gives
+// a key stage too for the parts of the rows it owns.
+template <bool kSplit>
 struct TileSmem {
+    static constexpr int kKStages = kSplit ? 2 : 3;
     static constexpr int q = 0;
-    static constexpr int k = q + kTileBytes;
-    static constexpr int v = k + kKStages * kTileBytes;
-    static constexpr int stage = v + kVStages * kTileBytes;  // 4 KB per softmax warp: its output rows
+    static constexpr int v = q + kTileBytes;
+    static constexpr int k = v + kVStages * kTileBytes;
+    static constexpr int stage = k + 3 * kTileBytes;  // 4 KB per softmax warp: its output rows
+    // kSplit: O of the parts, [source CTA][row this CTA owns][64] floats (16-byte piece
+    // c of a row at c ^ (row & 15)), each divided by its sum
+    static constexpr int part = k + kKStages * kTileBytes;
+    static_assert(!kSplit || part + kBlockM * 256 == stage + kTileBytes, "parts fill the space");
     static constexpr int bars = stage + kTileBytes;
     static constexpr int kQ = 0;
     static constexpr int kKFull = 1;
@@ -134,15 +143,13 @@ struct TileSmem {
     static constexpr int misc = bars + kNumBars * 8;  // the bounded waits' block (attn_kernel.cuh Smem::misc)
     static constexpr int records = (misc + 48 + 15) / 16 * 16;
     static constexpr int answer = records + 2 * 64;
-    static constexpr int total = answer + 16;
-    static constexpr int alloc = total;
-    // a split unit's partial rows, [66][128] floats (64 of O, max, sum), over the K ring
-    static constexpr int part = k;
-    static_assert(66 * 128 * 4 <= kKStages * kTileBytes, "partial rows");
+    static constexpr int lse = answer + 16;  // kSplit: log2 of the parts' sums, [source CTA][row]
+    static constexpr int alloc = lse + (kSplit ? kBlockM * 4 : 0);
     static_assert(2 * (alloc + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 constexpr int kTmemColsTile = 256;  // S [0, 128), P [128, 192), O [192, 256)
 constexpr int kTP = 128, kTO = 192;
+constexpr int kTmemDone = 128 + 2 * 32;  // the softmax warps, the MMA warp and the one that releases TMEM
 
 struct Maps {
     CUtensorMap q, k, v;    // boxes of 128 rows
@@ -150,36 +157,39 @@ struct Maps {
     CUtensorMap out;        // boxes of 32 rows (out_boxes)
 };
 
-// Merge of row `row` of a split unit, the `part_idx`-th of `split` column ranges, into
-// `out` (the row's 64 values) if it is a real row; parts are folded in rank order,
-// so the result does not depend on their timing.
+// Row `row` of a split unit from its parts in this CTA's shared memory, columns
+// [c0, c0 + 64 / split) of it into `out` if it is a real row: sum_r w_r O_r / sum_r w_r
+// with w_r = 2^(lse_r - max lse), in rank order, so the result does not depend on the
+// parts' timing. (The log's rounding is one more of the size of the scores' own.)
 template <typename T>
-__device__ __forceinline__ void merge_parts(uint32_t part, int split, int row, int part_idx, bool real, T* out) {
-    const int width = kHeadDim / split, c0 = part_idx * width;  // this thread's columns: 32, 16 or 8
-    float m = -INFINITY;
-    for (int r = 0; r < split; ++r) m = fmaxf(m, ld_cluster_f32(map_to_rank(part + 512u * 64 + 4u * row, r)));
-    float l = 0.f, f[kMaxSplit];
+__device__ __forceinline__ void merge_parts(uint32_t part, uint32_t lse, int split, int row, int c0, bool real, T* out) {
+    const int rows = kBlockM / split;
+    float m = -INFINITY, l = 0.f, f[kMaxSplit];
 #pragma unroll
     for (int r = 0; r < kMaxSplit; ++r) {
-        f[r] = 0.f;
-        if (r >= split) continue;
-        const uint32_t at = map_to_rank(part + 4u * row, r);
-        const float mr = ld_cluster_f32(at + 512u * 64);
-        f[r] = mr == -INFINITY ? 0.f : ex2_approx(mr - m);
-        l = fmaf(ld_cluster_f32(at + 512u * 65), f[r], l);
+        f[r] = r < split ? ld_shared_f32(lse + 4 * (r * rows + row)) : -INFINITY;
+        m = fmaxf(m, f[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxSplit; ++r) {
+        f[r] = f[r] == -INFINITY ? 0.f : ex2_approx(f[r] - m);
+        l += f[r];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-    for (int c = c0; c < c0 + width; c += 8) {
+    for (int c = c0; c < c0 + kHeadDim / split; c += 8) {
         float acc[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll
         for (int r = 0; r < kMaxSplit; ++r) {
             if (r >= split) continue;
-            const uint32_t at = map_to_rank(part + 4u * row, r);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(ld_cluster_f32(at + 512u * (c + e)), f[r], acc[e]);
+            const int at = r * rows + row;
+            const float4 a = ld_shared_v4f32(part + 256 * at + 16 * ((c >> 2) ^ (at & 15)));
+            const float4 b = ld_shared_v4f32(part + 256 * at + 16 * (((c >> 2) + 1) ^ (at & 15)));
+            acc[0] = fmaf(a.x, f[r], acc[0]), acc[1] = fmaf(a.y, f[r], acc[1]), acc[2] = fmaf(a.z, f[r], acc[2]);
+            acc[3] = fmaf(a.w, f[r], acc[3]), acc[4] = fmaf(b.x, f[r], acc[4]), acc[5] = fmaf(b.y, f[r], acc[5]);
+            acc[6] = fmaf(b.z, f[r], acc[6]), acc[7] = fmaf(b.w, f[r], acc[7]);
         }
         if (real)
             *reinterpret_cast<uint4*>(out + c) =
@@ -188,23 +198,24 @@ __device__ __forceinline__ void merge_parts(uint32_t part, int split, int row, i
     }
 }
 
-// A unit (row block fastest, then head group, then window): queries [row0, row0 +
-// n) of heads [h, h + pack) of window b, and this CTA's share of its tiles, [t0, t1).
+// A unit, by its place in the grid (row block, head group, window): queries [row0,
+// row0 + n) of heads [h, h + pack) of window b, which read key head hk, and this CTA's
+// share of its tiles, [t0, t1).
 struct Unit {
-    int b, h, row0, n, t0, t1;
+    int b, h, hk, row0, n, t0, t1;
     Columns c;
 };
 
-__device__ __forceinline__ Unit make_unit(const Params& p, int unit, int split, int rank) {
-    const int groups = p.heads / p.pack, bg = unit / p.row_blocks;
+__device__ __forceinline__ Unit make_unit(const Params& p, int block, int group, int b, int split_log2, int rank) {
     Unit u;
-    u.b = bg / groups;
-    u.h = (bg - u.b * groups) * p.pack;
-    u.row0 = (unit - bg * p.row_blocks) * p.queries;
+    u.b = b;
+    u.h = group * p.pack;
+    u.hk = p.pack > 1 ? group : group / (p.heads / p.kv_heads);
+    u.row0 = block * p.queries;
     u.n = min(p.queries, p.q_len - u.row0);
     u.c = Columns(p, u.b, u.row0, u.n);
     const int tiles = (u.c.total() + kBlockN - 1) / kBlockN;
-    const int per = (tiles + split - 1) / split;
+    const int per = (tiles + (1 << split_log2) - 1) >> split_log2;
     u.t0 = min(tiles, rank * per);
     u.t1 = min(tiles, u.t0 + per);
     return u;
@@ -218,13 +229,13 @@ __device__ __forceinline__ Unit make_unit(const Params& p, int unit, int split, 
 constexpr int kRecords = 2;
 constexpr int kRecordReaders = 6;  // MMA, TMA, four softmax warps
 
-__device__ __forceinline__ void store_record(uint32_t at, const Unit& u, int hk) {
+__device__ __forceinline__ void store_record(uint32_t at, const Unit& u) {
     st_shared_v4(at, make_int4(u.b, u.h, u.row0, u.n));
     st_shared_v4(at + 16, make_int4(u.t0, u.t1, u.c.p0, u.c.kv_end));
     st_shared_v4(at + 32, make_int4(u.c.begin, u.c.n_win, u.c.s0, u.c.n_sink));
     const int pad = u.c.s0 > u.c.n_win ? u.c.n_win / kBlockN - u.t0 : -1;
     const int end = u.c.total() % kBlockN != 0 ? u.c.total() / kBlockN - u.t0 : -1;
-    st_shared_v4(at + 48, make_int4(hk, pad, end, 1));
+    st_shared_v4(at + 48, make_int4(u.hk, pad, end, 1));
 }
 
 // Columns [x0, x0 + 128), some of them sinks, of the keys or values of a unit
@@ -285,16 +296,18 @@ __device__ __forceinline__ void store_box(uint32_t stage, const CUtensorMap* map
 // The grid has a CTA (or cluster) per unit; a CTA that finishes early takes over
 // the units of CTAs that have not started, so that the next unit's copies and
 // first scores run under the present one's last tiles and epilogue.
-template <typename T>
+template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __grid_constant__ Maps maps, const Params p) {
-    using S = TileSmem;
+    using S = TileSmem<kSplit>;
+    constexpr int kKStages = S::kKStages;
     extern __shared__ __align__(1024) uint8_t smem[];  // the tiles' swizzle repeats every 1024 bytes
     const uint32_t sbase = smem_u32(smem);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::bars);
     const WaitCtl ctl{sbase + S::misc};
     const auto bar = [&](int idx) { return sbase + S::bars + 8u * idx; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    const int split = kSplit ? static_cast<int>(cluster_nctarank()) : 1, rank = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+    const int split_log2 = kSplit ? 31 - __clz(split) : 0;
     grid_launch_dependents();
 
     if (threadIdx.x == 0) {
@@ -334,6 +347,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if constexpr (kSplit) cluster_arrive();  // this CTA runs: its shared memory may be stored to (waited for before the first store)
     grid_dependency_wait();
     const uint32_t tmem = *reinterpret_cast<uint32_t*>(smem + S::misc);
 
@@ -372,7 +386,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
         rs.kv_end = 0;
         rs.s_parity = 0;
         rs.pv_parity = 0;
-        bool ok = true;
+        bool ok = true, all_run = !kSplit;
         for (int i = 0; ok && record_wait(i, FDS_STATUS_TIMEOUT_SOFTMAX); ++i) {
             const int4 un = ld_shared_v4(record(i) + 16);  // t0, t1, p0, kv_end
             const int t1 = un.y;
@@ -414,7 +428,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
 #pragma unroll
                 for (int e = 0; e < 64; ++e) o[e] = 0;
             }
-            if (split == 1) {
+            if constexpr (!kSplit) {
                 const int4 at = ld_shared_v4(record(i));  // b, h, row0, n: not held in registers over the tiles
                 uint32_t w[32];
 #pragma unroll
@@ -433,29 +447,33 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
                         *reinterpret_cast<uint4*>(to + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
                 }
             } else {
-                const uint32_t part = sbase + S::part + 4u * row;
+                cluster_wait();
+                all_run = true;
+                // to the CTA that owns the row (its row of it: row % (128 / split))
+                const int own = kBlockM >> split_log2, at = rank * own + (row & (own - 1)), owner = row >> (7 - split_log2);
+                const uint32_t to = map_to_rank(sbase + S::part + 256 * at, owner);
 #pragma unroll
-                for (int e = 0; e < 64; ++e) st_shared_f32(part + 512u * e, __uint_as_float(o[e]));
-                st_shared_f32(part + 512u * 64, rs.m_run);
-                st_shared_f32(part + 512u * 65, none ? 0.f : rs.l_run);
+                for (int c = 0; c < 16; ++c)
+                    st_cluster_v4f32(to + 16 * (c ^ (at & 15)), __uint_as_float(o[4 * c]) * inv, __uint_as_float(o[4 * c + 1]) * inv,
+                                     __uint_as_float(o[4 * c + 2]) * inv, __uint_as_float(o[4 * c + 3]) * inv);
+                st_cluster_f32(map_to_rank(sbase + S::lse + 4 * at, owner), none ? -INFINITY : rs.m_run + __log2f(rs.l_run));
             }
-            if (split == 1) record_release(i);
+            if constexpr (!kSplit) record_release(i);
         }
         if (lane == 0) bulk_wait_all();  // the output boxes are written
         __syncwarp();
         tc_fence_before();
-        named_barrier_sync(1, kTileThreads);
-        if (split > 1) {
-            cluster_sync_all();
+        named_barrier_arrive(1, kTmemDone);
+        if constexpr (kSplit) {
+            if (!all_run) cluster_wait();  // (a timeout before the unit was known)
+            cluster_arrive();
+            cluster_wait();  // every part is in place
             const int4 at = ld_shared_v4(record(0));  // (the end of the list is in the other slot)
-            // CTA `rank` takes rows [128 rank / split, ..), `split` threads a row
-            const int tid = static_cast<int>(threadIdx.x) - 128;
-            const int mrow = rank * (kBlockM / split) + tid / split, mq = mrow / p.pack;
-            merge_parts<T>(sbase + S::part, split, mrow, tid % split, mq < at.w,
+            const int own = kBlockM >> split_log2, tid = static_cast<int>(threadIdx.x) - 128;
+            const int mine = tid & (own - 1), mrow = rank * own + mine, mq = mrow / p.pack;
+            merge_parts<T>(sbase + S::part, sbase + S::lse, split, mine, (tid >> (7 - split_log2)) * (kHeadDim >> split_log2), ok && all_run && mq < at.w,
                            static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + mq) * p.out_stride[1] +
                                (at.y + mrow - mq * p.pack) * p.out_stride[2]);
-            __syncwarp();
-            cluster_sync_all();  // no CTA leaves while its parts are read
         }
     } else {
         setmaxnreg_dec<kControlRegs>();
@@ -600,21 +618,21 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
             // launch control hands them out as they are asked for, so SMs of
             // different speeds share the units as if each had its own CTA.
             constexpr int err = FDS_STATUS_TIMEOUT_LOAD;
-            int unit = static_cast<int>(blockIdx.x) / split;
+            int block[3] = {static_cast<int>(blockIdx.x) >> split_log2, static_cast<int>(blockIdx.y), static_cast<int>(blockIdx.z)};
             bool ok = true, more = true;
             for (int i = 0; ok; ++i) {
                 if (i >= kRecords) ok = warp_wait(bar(S::kRecEmpty + i % kRecords), (i / kRecords - 1) & 1, ctl, err);
                 if (!ok) break;
                 if (more) {
-                    const Unit un = make_unit(p, unit, split, rank);
-                    if (lane == 0) store_record(record(i), un, un.h / (p.heads / p.kv_heads));
+                    const Unit un = make_unit(p, block[0], block[1], block[2], split_log2, rank);
+                    if (lane == 0) store_record(record(i), un);
                 } else if (lane == 0) {
                     st_shared_volatile_u32(record(i) + 60, 0);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(S::kRecFull + i % kRecords));
                 if (!more) break;
-                if (split > 1) {  // a cluster holds one unit
+                if constexpr (kSplit) {  // a cluster holds one unit
                     more = false;
                     continue;
                 }
@@ -629,22 +647,25 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
                     __syncwarp();
                     break;
                 }
-                more = launch_control_answer(sbase + S::answer, unit);
+                more = launch_control_answer(sbase + S::answer, block);
                 fence_proxy_async_smem();  // the answer is read before the next one is written
                 __syncwarp();
             }
         }
         __syncwarp();
         tc_fence_before();
-        named_barrier_sync(1, kTileThreads);
+        if constexpr (kSplit) {
+            cluster_wait();
+            cluster_arrive();
+        }
+        // TMEM is released once the MMAs have completed and the softmax warps have read O
+        if (warp == 0) named_barrier_arrive(1, kTmemDone);
         if (warp == 2) {
+            named_barrier_sync(1, kTmemDone);
             tc_fence_after();
             tmem_dealloc(tmem, kTmemColsTile);
         }
-        if (split > 1) {
-            cluster_sync_all();
-            cluster_sync_all();
-        }
+        if constexpr (kSplit) cluster_wait();
     }
 }
 
@@ -657,9 +678,10 @@ constexpr int kStepKeys = 32;     // keys of a block
 constexpr int kStepStages = 3;    // blocks in a warp's ring
 constexpr int kBlockBytes = kStepKeys * 128;                       // keys or values of a block
 constexpr int kStepWarpBytes = kStepStages * 2 * kBlockBytes;
-constexpr int kStepSmem = kStepWarps * kStepWarpBytes;
 constexpr int kPartFloats = 66;   // a row's 64 of O, max, sum
-static_assert(kStepWarps * kStepRows * kPartFloats * 4 <= kStepSmem, "partial rows over the rings");
+constexpr int kStepRings = kStepWarps * kStepWarpBytes;
+constexpr int kStepSmem = kStepRings + kStepRows * kPartFloats * 4;  // and a cluster's parts of the rows this CTA owns
+static_assert(kStepWarps * kStepRows * kPartFloats * 4 <= kStepRings, "partial rows over the rings");
 
 // 16 bytes, or zeros, asynchronously into shared memory.
 __device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool on) {
@@ -705,11 +727,12 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uin
 template <typename T, int kHalves, bool kMulti>
 __global__ void __launch_bounds__(kStepThreads) window_step_kernel(const Params p) {
     extern __shared__ __align__(128) uint8_t step_smem[];
+    const int split = static_cast<int>(gridDim.x), rank = static_cast<int>(blockIdx.x);
+    if (split > 1) cluster_arrive();  // this CTA runs: its shared memory may be stored to
     grid_launch_dependents();
     grid_dependency_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;  // fragment row (or key, or value column) and column pair
-    const int split = static_cast<int>(gridDim.x), rank = static_cast<int>(blockIdx.x);
     const int hk = blockIdx.y, b = blockIdx.z;
     const int group = p.heads / p.kv_heads;
     const int n_rows = p.q_len * group;
@@ -848,35 +871,56 @@ __global__ void __launch_bounds__(kStepThreads) window_step_kernel(const Params 
         if (t == 0) row[64] = m[h], row[65] = l[h];
     }
     __syncthreads();
-    if (split > 1) cluster_sync_all();
-    // merge all shares in order; the CTAs of the cluster take the rows' columns in turn
-    for (int i = rank * kStepThreads + static_cast<int>(threadIdx.x); i < n_rows * 64; i += split * kStepThreads) {
-        const int r = i >> 6, c = i & 63;
-        const uint32_t at = smem_u32(part + r * kPartFloats);
-        float mm = -INFINITY;
-        for (int k = 0; k < split; ++k) {
-            const uint32_t a = map_to_rank(at + 4u * 64, k);
-#pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) mm = fmaxf(mm, ld_cluster_f32(a + 4u * w * kStepRows * kPartFloats));
-        }
-        const float base = mm == -INFINITY ? 0.f : mm;
-        float acc = 0.f, sum = 0.f;
-        for (int k = 0; k < split; ++k) {
-            const uint32_t a = map_to_rank(at, k);
-#pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) {
-                const uint32_t aw = a + 4u * w * kStepRows * kPartFloats;
-                const float f = ex2_approx(ld_cluster_f32(aw + 4u * 64) - base);
-                acc = fmaf(ld_cluster_f32(aw + 4u * c), f, acc);
-                sum = fmaf(ld_cluster_f32(aw + 4u * 65), f, sum);
-            }
-        }
+    const auto store = [&](int r, int c, float acc, float sum) {
         T* out = static_cast<T*>(p.out) + b * p.out_stride[0] + (r / group) * p.out_stride[1] +
                  (hk * group + r % group) * p.out_stride[2];
         out[c] = static_cast<T>(sum == 0.f ? 0.f : acc / sum);
+    };
+    // the warps' shares in order, then (a cluster) the CTAs' by the one that owns the
+    // row, row % split: the others store theirs into its shared memory
+    if (split > 1) cluster_wait();
+    float* owned = reinterpret_cast<float*>(step_smem + kStepRings);  // [row / split][source][66]
+    for (int i = threadIdx.x; i < n_rows * 64; i += kStepThreads) {
+        const int r = i >> 6, c = i & 63;
+        const float* from = part + r * kPartFloats;
+        float mm = -INFINITY, acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kStepWarps; ++w) mm = fmaxf(mm, from[w * kStepRows * kPartFloats + 64]);
+        const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+        for (int w = 0; w < kStepWarps; ++w) {
+            const float* fw = from + w * kStepRows * kPartFloats;
+            const float f = ex2_approx(fw[64] - base);
+            acc = fmaf(fw[c], f, acc);
+            sum = fmaf(fw[65], f, sum);
+        }
+        if (split == 1) {
+            store(r, c, acc, sum);
+        } else {
+            const int own = r / split;
+            const uint32_t to = map_to_rank(smem_u32(owned + (own * split + rank) * kPartFloats), r - own * split);
+            st_cluster_f32(to + 4u * c, acc);
+            if (c == 0) st_cluster_f32(to + 4u * 64, mm);
+            if (c == 1) st_cluster_f32(to + 4u * 65, sum);
+        }
     }
+    if (split == 1) return;
     __syncwarp();
-    if (split > 1) cluster_sync_all();  // no CTA leaves while its parts are read
+    cluster_sync_all();
+    for (int i = threadIdx.x; i < n_rows * 64; i += kStepThreads) {
+        const int own = i >> 6, r = own * split + rank, c = i & 63;
+        if (r >= n_rows) break;
+        const float* from = owned + own * split * kPartFloats;
+        float mm = -INFINITY, acc = 0.f, sum = 0.f;
+        for (int k = 0; k < split; ++k) mm = fmaxf(mm, from[k * kPartFloats + 64]);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        for (int k = 0; k < split; ++k) {
+            const float f = ex2_approx(from[k * kPartFloats + 64] - base);
+            acc = fmaf(from[k * kPartFloats + c], f, acc);
+            sum = fmaf(from[k * kPartFloats + 65], f, sum);
+        }
+        store(r, c, acc, sum);
+    }
 }
 
 }  // namespace window
