@@ -69,6 +69,28 @@ int64_t most_keys(const Params& p, int rows) {
     return std::min<int64_t>(p.k_len, static_cast<int64_t>(p.left) + p.right + rows + p.sinks);
 }
 
+// CTAs (1, 2, 4 or 8, a cluster) that a unit's tiles are dealt to: the split that
+// should finish first, of those whose clusters are all resident at once. The constants
+// are microseconds on a B200 (77 queries, 4 - 128 units, 2 - 24 tiles; within 10 % but
+// for a few): a launch, more for a cluster's merge, and a tile of each CTA, dearer
+// where CTAs share a pair of SMs, then one. E.g. 12 units: 3 tiles 8.1 us whole, 8.3
+// in four; 8 tiles 13.0, 8.9 in four; 36 units: 4 tiles 9.7, 9.1 in two, 9.9 in four;
+// 16 tiles 23.4, 15.5, 14.0. Eight CTAs a cluster fit up to four thirds of the SMs (36
+// units of 4 tiles: 16.9 us, in two waves).
+int choose_split(int64_t units, int64_t tiles, int64_t sms) {
+    int best = 1;
+    double best_cost = 1e30;
+    for (int split = 1; split <= fds::window::kMaxSplit; split *= 2) {
+        const int64_t ctas = units * split;
+        if (split > 1 && ctas > (split == 8 ? sms * 4 / 3 : 2 * sms)) break;
+        const int step = ctas <= sms / 2 ? 0 : (ctas <= sms ? 1 : 2);
+        const double launch[] = {5.2, 5.9, 5.9}, merge[] = {1.8, 2.6, 2.8}, tile[] = {1.05, 1.43, 1.67};
+        const double cost = launch[step] + (split > 1 ? merge[step] : 0.) + static_cast<double>((tiles + split - 1) / split) * tile[step];
+        if (cost < best_cost) best_cost = cost, best = split;
+    }
+    return best;
+}
+
 template <typename T, bool kSplit>
 int launch_units(const fds::window::Maps& maps, const Params& p, int batch, int split, cudaStream_t stream) {
     auto kern = fds::window::window_tile_kernel<T, kSplit>;
@@ -104,23 +126,21 @@ int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream)
     if (p.out_boxes && (rc = make_heads_map(&maps.out, a->out, a->dtype, p.heads, p.q_len, a->batch, p.out_stride, 32 / p.pack, p.pack)) != FDS_OK)
         return rc;
     const int64_t units = static_cast<int64_t>(a->batch) * (p.heads / p.pack) * p.row_blocks;
-    // A unit's tiles are dealt to a cluster while that still fills idle SMs
-    // (two CTAs each) and leaves every CTA two tiles.
     const int64_t tiles = (most_keys(p, p.queries) + fds::kBlockN - 1) / fds::kBlockN;
-    int split = 1;
-    while (split < fds::window::kMaxSplit && units * split * 2 <= 2 * sms && tiles >= 4 * split) split *= 2;
+    const int split = choose_split(units, tiles, sms);
     if (p.heads / p.pack > 65535) return set_error(FDS_ERR_INVALID_ARGUMENT, "more than 65535 heads");
     return split > 1 ? launch_units<T, true>(maps, p, a->batch, split, stream) : launch_units<T, false>(maps, p, a->batch, 1, stream);
 }
 
 template <typename T, int kHalves, bool kMulti>
 int launch_step(const Params& p, int batch, int sms, cudaStream_t stream) {
-    // The keys of a (window, key head) are dealt to the warps of a cluster while
-    // that leaves every warp a block of 32 keys and at most 2 CTAs per SM.
+    // The keys of a (window, key head) are dealt to the warps of a cluster while that
+    // leaves most warps a block of 32 keys and at most 2 CTAs per SM (12 heads, 504 keys:
+    // 3.75 us in four CTAs, 4.2 in two).
     const int64_t units = static_cast<int64_t>(batch) * p.kv_heads, keys = most_keys(p, p.q_len);
     int split = 1;
     while (split < fds::window::kMaxSplit && units * split * 2 <= 2 * sms &&
-           keys >= 2 * split * fds::window::kStepWarps * fds::window::kStepKeys)
+           keys >= split * fds::window::kStepWarps * fds::window::kStepKeys)
         split *= 2;
     auto kern = fds::window::window_step_kernel<T, kHalves, kMulti>;
     static std::atomic<uint64_t> smem_set{0};
