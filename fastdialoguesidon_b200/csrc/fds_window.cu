@@ -108,8 +108,8 @@ int launch_units(const fds::window::Maps& maps, const Params& p, int batch, int 
 template <typename T>
 int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream) {
     // the heads of a key head share units, so that its keys are read once for them
-    const int group = p.heads / p.kv_heads;
-    p.pack = group <= fds::kBlockM ? group : 1;
+    p.group = p.heads / p.kv_heads;
+    p.pack = p.group <= fds::kBlockM ? p.group : 1;
     p.queries = fds::kBlockM / p.pack;
     fds::window::Maps maps;
     int rc;

@@ -62,9 +62,9 @@ struct Params {
     int32_t debug_flags;
     int32_t heads, kv_heads, q_len, k_len;
     int32_t left, right, sinks;
-    // tile kernel: `pack` heads of a unit (those of one key head, or 1) and
+    // tile kernel: `pack` heads of a unit (the `group` of one key head, or 1) and
     // `queries` = 128 / pack of each; row r of a unit is query r / pack, head r % pack
-    int32_t pack, queries;
+    int32_t group, pack, queries;
     int32_t row_blocks;  // ceil(q_len / queries)
     int32_t out_boxes;   // pack divides 32: a warp's output rows are a box of heads x queries
     float scale_log2;
@@ -160,37 +160,32 @@ struct Maps {
 // Row `row` of a split unit from its parts in this CTA's shared memory, columns
 // [c0, c0 + 64 / split) of it into `out` if it is a real row: sum_r w_r O_r / sum_r w_r
 // with w_r = 2^(lse_r - max lse), in rank order, so the result does not depend on the
-// parts' timing. (The log's rounding is one more of the size of the scores' own.)
+// parts' timing. (The log's rounding is one more of the size of the scores' own. The
+// loops are rolled: this runs once, and fetching its instructions is most of it.)
 template <typename T>
 __device__ __forceinline__ void merge_parts(uint32_t part, uint32_t lse, int split, int row, int c0, bool real, T* out) {
     const int rows = kBlockM / split;
-    float m = -INFINITY, l = 0.f, f[kMaxSplit];
-#pragma unroll
-    for (int r = 0; r < kMaxSplit; ++r) {
-        f[r] = r < split ? ld_shared_f32(lse + 4 * (r * rows + row)) : -INFINITY;
-        m = fmaxf(m, f[r]);
-    }
-#pragma unroll
-    for (int r = 0; r < kMaxSplit; ++r) {
-        f[r] = f[r] == -INFINITY ? 0.f : ex2_approx(f[r] - m);
-        l += f[r];
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float m = -INFINITY;
+#pragma unroll 2
+    for (int r = 0; r < split; ++r) m = fmaxf(m, ld_shared_f32(lse + 4 * (r * rows + row)));
+    if (m == -INFINITY) m = 0.f;
 #pragma unroll 1
     for (int c = c0; c < c0 + kHeadDim / split; c += 8) {
-        float acc[8];
+        float acc[8], l = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-#pragma unroll
-        for (int r = 0; r < kMaxSplit; ++r) {
-            if (r >= split) continue;
+#pragma unroll 2
+        for (int r = 0; r < split; ++r) {
             const int at = r * rows + row;
+            const float f = ex2_approx(ld_shared_f32(lse + 4 * at) - m);
             const float4 a = ld_shared_v4f32(part + 256 * at + 16 * ((c >> 2) ^ (at & 15)));
             const float4 b = ld_shared_v4f32(part + 256 * at + 16 * (((c >> 2) + 1) ^ (at & 15)));
-            acc[0] = fmaf(a.x, f[r], acc[0]), acc[1] = fmaf(a.y, f[r], acc[1]), acc[2] = fmaf(a.z, f[r], acc[2]);
-            acc[3] = fmaf(a.w, f[r], acc[3]), acc[4] = fmaf(b.x, f[r], acc[4]), acc[5] = fmaf(b.y, f[r], acc[5]);
-            acc[6] = fmaf(b.z, f[r], acc[6]), acc[7] = fmaf(b.w, f[r], acc[7]);
+            l += f;
+            acc[0] = fmaf(a.x, f, acc[0]), acc[1] = fmaf(a.y, f, acc[1]), acc[2] = fmaf(a.z, f, acc[2]);
+            acc[3] = fmaf(a.w, f, acc[3]), acc[4] = fmaf(b.x, f, acc[4]), acc[5] = fmaf(b.y, f, acc[5]);
+            acc[6] = fmaf(b.z, f, acc[6]), acc[7] = fmaf(b.w, f, acc[7]);
         }
+        const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);  // l: 1 to 8 and the smaller weights
         if (real)
             *reinterpret_cast<uint4*>(out + c) =
                 make_uint4(norm::pack2<T>(acc[0] * inv, acc[1] * inv), norm::pack2<T>(acc[2] * inv, acc[3] * inv),
@@ -210,7 +205,7 @@ __device__ __forceinline__ Unit make_unit(const Params& p, int block, int group,
     Unit u;
     u.b = b;
     u.h = group * p.pack;
-    u.hk = p.pack > 1 ? group : group / (p.heads / p.kv_heads);
+    u.hk = p.pack == p.group ? group : group / p.group;
     u.row0 = block * p.queries;
     u.n = min(p.queries, p.q_len - u.row0);
     u.c = Columns(p, u.b, u.row0, u.n);
@@ -467,13 +462,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
         if constexpr (kSplit) {
             if (!all_run) cluster_wait();  // (a timeout before the unit was known)
             cluster_arrive();
-            cluster_wait();  // every part is in place
             const int4 at = ld_shared_v4(record(0));  // (the end of the list is in the other slot)
             const int own = kBlockM >> split_log2, tid = static_cast<int>(threadIdx.x) - 128;
             const int mine = tid & (own - 1), mrow = rank * own + mine, mq = mrow / p.pack;
-            merge_parts<T>(sbase + S::part, sbase + S::lse, split, mine, (tid >> (7 - split_log2)) * (kHeadDim >> split_log2), ok && all_run && mq < at.w,
-                           static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + mq) * p.out_stride[1] +
-                               (at.y + mrow - mq * p.pack) * p.out_stride[2]);
+            T* to = static_cast<T*>(p.out) + at.x * p.out_stride[0] + (at.z + mq) * p.out_stride[1] +
+                    (at.y + mrow - mq * p.pack) * p.out_stride[2];
+            cluster_wait();  // every part is in place
+            merge_parts<T>(sbase + S::part, sbase + S::lse, split, mine, (tid >> (7 - split_log2)) * (kHeadDim >> split_log2),
+                           ok && all_run && mq < at.w, to);
         }
     } else {
         setmaxnreg_dec<kControlRegs>();
