@@ -26,9 +26,10 @@ int launch(Params& p, int threads, int per_sm, int sms, cudaStream_t stream) {
 }
 
 // A CTA as wide as the row: 8 columns a thread up to 4096, 16 or 32 beyond. The
-// grid is what the SMs hold at once (16 warps each at 128 registers); four rows at a time once a CTA has two or more (3000 x 768
-// fp32 stream: 6.9 us against 8.3 us row by row, 6000 x 768: 13.9 against 16.9),
-// single rows below, which are bound by one row's latency.
+// grid is what the SMs hold at once (16 warps each at 128 registers); four rows at a
+// time once a CTA has two or more (3000 x 768 fp32 stream: 6.9 us against 8.3 us row
+// by row, 6000 x 768: 13.9 against 16.9), single rows below, which are bound by one
+// row's latency.
 template <typename T, int kMode, bool kXf32, bool kQuant>
 int launch_shape(Params& p, int sms, cudaStream_t s) {
     const int nch = p.c <= 4096 ? 1 : (p.c <= 8192 ? 2 : 4);

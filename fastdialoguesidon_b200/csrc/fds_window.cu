@@ -115,19 +115,22 @@ int launch_tile(const FdsWindowArgs* a, Params& p, int sms, cudaStream_t stream)
     int rc;
     if ((rc = make_heads_map(&maps.q, a->q, a->dtype, p.heads, p.q_len, a->batch, p.q_stride, p.queries, p.pack)) != FDS_OK ||
         (rc = make_heads_map(&maps.k, a->k, a->dtype, p.kv_heads, p.k_len, a->batch, p.k_stride, fds::kBlockN)) != FDS_OK ||
-        (rc = make_heads_map(&maps.v, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, fds::kBlockN)) != FDS_OK ||
-        (rc = make_heads_map(&maps.k8, a->k, a->dtype, p.kv_heads, p.k_len, a->batch, p.k_stride, 8)) != FDS_OK ||
-        (rc = make_heads_map(&maps.v8, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, 8)) != FDS_OK)
+        (rc = make_heads_map(&maps.v, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, fds::kBlockN)) != FDS_OK)
+        return rc;
+    // (a map costs the host a third of a microsecond: only those the launch reads)
+    maps.k8 = maps.k, maps.v8 = maps.v, maps.out = maps.q;
+    if (p.sinks > 0 &&
+        ((rc = make_heads_map(&maps.k8, a->k, a->dtype, p.kv_heads, p.k_len, a->batch, p.k_stride, 8)) != FDS_OK ||
+         (rc = make_heads_map(&maps.v8, a->v, a->dtype, p.kv_heads, p.k_len, a->batch, p.v_stride, 8)) != FDS_OK))
         return rc;
     p.row_blocks = (p.q_len + p.queries - 1) / p.queries;
-    // a warp's 32 output rows are whole queries: one box each (else a row per thread)
-    p.out_boxes = 32 % p.pack == 0;
-    maps.out = maps.q;
-    if (p.out_boxes && (rc = make_heads_map(&maps.out, a->out, a->dtype, p.heads, p.q_len, a->batch, p.out_stride, 32 / p.pack, p.pack)) != FDS_OK)
-        return rc;
     const int64_t units = static_cast<int64_t>(a->batch) * (p.heads / p.pack) * p.row_blocks;
     const int64_t tiles = (most_keys(p, p.queries) + fds::kBlockN - 1) / fds::kBlockN;
     const int split = choose_split(units, tiles, sms);
+    // a warp's 32 output rows are whole queries: one box each (else a row per thread)
+    p.out_boxes = split == 1 && 32 % p.pack == 0;
+    if (p.out_boxes && (rc = make_heads_map(&maps.out, a->out, a->dtype, p.heads, p.q_len, a->batch, p.out_stride, 32 / p.pack, p.pack)) != FDS_OK)
+        return rc;
     if (p.heads / p.pack > 65535) return set_error(FDS_ERR_INVALID_ARGUMENT, "more than 65535 heads");
     return split > 1 ? launch_units<T, true>(maps, p, a->batch, split, stream) : launch_units<T, false>(maps, p, a->batch, 1, stream);
 }

@@ -8,7 +8,9 @@
 // epilogue, neighbours otherwise -- and walks k in 16-byte chunks per lane,
 // kUnroll chunks of each row in flight; A (a few rows) comes through L1. The
 // products are summed in 32-bit integers (dp4a), exactly, so the result does
-// not depend on the split of k over lanes.
+// not depend on the split of k over lanes. 768 -> 2304, one row: 1.95 us, as long as
+// an empty launch; 4096 -> 4096 in us (this / the 64-column tiles of gemm_kernel):
+// one row 4.3 / 13.4, eight rows 7.2 / 12.
 #pragma once
 
 #include <cstdint>

@@ -26,6 +26,11 @@
 //   that each warp fills and reads by itself (no CTA barrier), so that up to
 //   192 KB per SM are in flight while the present rows pass through their
 //   reductions.
+// 29777 x 1160, 16-bit stream: 52.7 us, 5.2 TB/s (71 without the ring; issue slots
+// 57 %, DRAM 55 % of its nominal rate); 6000 x 768, fp32 stream: 13.8 us; one row:
+// 2.8 us, 1.9 of which an empty launch takes. A warp per row instead, its vectors
+// read where they are used, is faster only while they stay in L1 and L2 (6000 x
+// 768: 13.0 us with one vector for all, 19.5 with five that come from DRAM).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -371,9 +371,9 @@ FDS_API int fds_residual_norm_fwd(const FdsResidualNormArgs* args, void* stream)
  * that sees none. q / out [batch, q_len, heads, 64], k / v [batch, k_len,
  * kv_heads, 64] with any strides (batch, row, head; multiples of 8 elements);
  * query head h reads key head h / (heads / kv_heads). Keys and values that no
- * query of its 128-row tile sees (unwritten cache rows, rows past kv_len) may hold anything,
- * infinities and NaN included. Up to 16 query rows per key head (q_len * heads /
- * kv_heads) run on a kernel without tensor cores, split over the keys.
+ * query of its 128-row tile sees (unwritten cache rows, rows past kv_len) may
+ * hold anything, infinities and NaN included. Up to 16 query rows per key head
+ * (q_len * heads / kv_heads) run on a kernel of their own, split over the keys.
  * No counterpart in the reference, whose windows end at 120 s
  * (triton/src/fds_triton/runtime.py:179).
  */
