@@ -37,8 +37,8 @@
 //   rows as warp-level 16 x 8 x 16 products (a 128-row tcgen05 tile would be
 //   seven-eighths empty, and the products are not what bounds it); the shares --
 //   4 warps of up to 8 CTAs of a cluster -- are merged the same way. 16 windows x
-//   16 heads x 1000 keys: 14.6 us, 4.6 TB/s; one window, 12 heads x 500 keys: 3.7,
-//   1.9 of which an empty launch takes.
+//   4 key heads x 4112 keys: 14.6 us, 4.6 TB/s; one window, 12 heads x 1004 keys:
+//   3.7, 1.9 of which an empty launch takes.
 //
 // Keys and values that no row of a unit sees may hold anything (a cache's
 // unwritten rows): their scores are replaced, and their value rows are zeroed
