@@ -117,7 +117,8 @@ struct Params {
     int32_t seq_len;          // kRope: position = row % seq_len
     int32_t rope_cols;        // kRope: columns [0, rope_cols) are rotated
     int32_t tiles_n;          // ceil(N / BN)
-    int32_t tiles;            // ceil(M / tile rows) * tiles_n
+    int32_t tiles;            // ceil(M / tile rows) * tiles_n, the cut ones counted by their pieces
+    int32_t whole, cut;       // kCut: tiles from `whole` on are cut into 2^cut pieces (1 or 2)
 };
 
 template <typename T>
@@ -209,6 +210,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int kb_n = kInt8 ? (p.k + kBKe - 1) / kBKe : p.k / kBKe;  // 8-bit: the last stage zero-filled past k
+    // The last tiles, where they would fill less than half a wave, as pieces of fewer
+    // columns: tile t's rows, first column and log2 of BN / its columns.
+    constexpr bool kCut = kInt8 && BN == 256 && kEpi != kRope;
+    struct Place {
+        int m_tile, n0, cut;
+    };
+    const auto place = [&](int t) {
+        if (!kCut || t < p.whole) return Place{t / p.tiles_n, (t % p.tiles_n) * BN, 0};
+        const int tile = p.whole + ((t - p.whole) >> p.cut), piece = (t - p.whole) & ((1 << p.cut) - 1);
+        return Place{tile / p.tiles_n, (tile % p.tiles_n) * BN + piece * (BN >> p.cut), p.cut};
+    };
 
     grid_launch_dependents();
     if (threadIdx.x == 0) {
@@ -265,8 +277,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int t = unit0; ok && t < p.tiles; t += units) {
             // this CTA's A rows and W rows of the tile
-            const int m0 = (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM;
-            const int n0 = (t % p.tiles_n) * BN + static_cast<int>(rank) * S::kBNc;
+            const Place at = place(t);
+            const int m0 = at.m_tile * kTileM + static_cast<int>(rank) * kBM;
+            const int n0 = at.n0 + static_cast<int>(rank) * (S::kBNc >> at.cut);
+            const uint32_t bytes = S::a_bytes + (S::b_bytes >> at.cut);
+            // the W rows: one box, those of a piece in quarter boxes (the map that the RoPE
+            // epilogue has for its cosines)
+            const auto load_w = [&](int st, int kb, auto load) {
+                const uint32_t to = sbase + S::b + st * S::b_bytes;
+                if (!kCut || at.cut == 0) {
+                    load(to, &map_b, kb * kBKe, n0);
+                } else {
+                    for (int j = 0; j < (4 >> at.cut); ++j)
+                        load(to + j * (S::b_bytes / 4), &map_cos, kb * kBKe, n0 + j * (S::kBNc / 4));
+                }
+            };
             for (int kb = 0; kb < kb_n; ++kb, ++g) {
                 const int st = g % S::kStages;
                 if (g >= S::kStages) {
@@ -277,13 +302,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if constexpr (kPair) {
                         // the even CTA's full barrier counts both CTAs' bytes; only it arms
                         const uint32_t fb = map_to_rank(bar(S::kFull + st), 0);
-                        if (rank == 0) mbar_arrive_expect_tx(bar(S::kFull + st), 2 * (S::a_bytes + S::b_bytes));
+                        if (rank == 0) mbar_arrive_expect_tx(bar(S::kFull + st), 2 * bytes);
                         tma_load_2d_pair(sbase + S::a + st * S::a_bytes, &map_a, fb, kb * kBKe, m0);
-                        tma_load_2d_pair(sbase + S::b + st * S::b_bytes, &map_b, fb, kb * kBKe, n0);
+                        load_w(st, kb, [&](uint32_t to, const CUtensorMap* map, int x, int y) { tma_load_2d_pair(to, map, fb, x, y); });
                     } else {
-                        mbar_arrive_expect_tx(bar(S::kFull + st), S::a_bytes + S::b_bytes);
+                        mbar_arrive_expect_tx(bar(S::kFull + st), bytes);
                         tma_load_2d(sbase + S::a + st * S::a_bytes, &map_a, bar(S::kFull + st), kb * kBKe, m0);
-                        tma_load_2d(sbase + S::b + st * S::b_bytes, &map_b, bar(S::kFull + st), kb * kBKe, n0);
+                        load_w(st, kb, [&](uint32_t to, const CUtensorMap* map, int x, int y) { tma_load_2d(to, map, bar(S::kFull + st), x, y); });
                     }
                 }
                 __syncwarp();
@@ -302,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1 && rank == 0) {
         // ------------------------------------------------ MMA issuer
-        constexpr uint32_t idesc = kInt8 ? idesc_s8(kTileM, BN) : idesc_f16(kTileM, BN, DTypeTraits<T>::kFormat, 0, 0);
+        constexpr uint32_t idesc_whole = kInt8 ? idesc_s8(kTileM, BN) : idesc_f16(kTileM, BN, DTypeTraits<T>::kFormat, 0, 0);
+        const uint32_t idesc_cut = kCut ? idesc_s8(kTileM, BN >> p.cut) : 0u;
         // completions go to both CTAs of a pair (their stages and accumulators)
         const auto commit = [&](int idx) {
             if constexpr (kPair) {
@@ -316,6 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true, issued = false;
         for (int t = unit0; ok && t < p.tiles; t += units, ++lt) {
             const int buf = lt & 1;
+            const uint32_t idesc = kCut && t >= p.whole ? idesc_cut : idesc_whole;
             if (lt >= 2) {  // the epilogue has read this accumulator out
                 ok = warp_wait(bar(S::kAccEmpty + buf), ((lt >> 1) - 1) & 1, ctl, FDS_STATUS_TIMEOUT_MMA);
                 if (!ok) break;
@@ -363,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int lt = 0;
         for (int t = unit0; t < p.tiles; t += units, ++lt) {
             // (the next tile's are in registers while the epilogue uses this one's)
-            const int n0 = (t % p.tiles_n) * BN;
+            const int n0 = place(t).n0;
             float w[BN / 32];
             T b[BN / 32];
 #pragma unroll
@@ -391,7 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         int lt = 0, armed = -1;
         bool ok = true;
         for (int t = unit0; ok && t < p.tiles; t += units, ++lt) {
-            const int m0 = (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM, n0 = (t % p.tiles_n) * BN;
+            const Place at = place(t);
+            const int m0 = at.m_tile * kTileM + static_cast<int>(rank) * kBM, n0 = at.n0;
             if (lt >= 1) {
                 ok = warp_wait(bar(S::kCsEmpty), (lt - 1) & 1, ctl, FDS_STATUS_TIMEOUT_LOAD);
                 if (!ok) break;
@@ -417,7 +445,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp >= kEpiWarp0 && warp < kEpiWarp0 + kActiveWarps) {
         // ------------------------------------------------ epilogue
         const int wq = warp & 3;                       // TMEM lane quarter
-        const int c_begin = ((warp - kEpiWarp0) >> 2) * kWarpCols;  // this warp's columns
         const int row = wq * 32 + lane;
         const uint32_t lane_addr = static_cast<uint32_t>(wq * 32) << 16;
         const uint32_t stg = sbase + S::stg + (warp - kEpiWarp0) * S::kStgBytes;
@@ -437,14 +464,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         // 8-bit operands: this row's scale in tile t, fetched a tile ahead
         const auto row_scale = [&](int t) {
-            const int m = t < p.tiles ? (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM + row : p.m;
+            const int m = t < p.tiles ? place(t).m_tile * kTileM + static_cast<int>(rank) * kBM + row : p.m;
             return m < p.m ? __ldg(p.a_scale + m) : 0.f;
         };
         float as_next = 0.f;
         if constexpr (kInt8) as_next = row_scale(unit0);
         for (int t = unit0; ok && t < p.tiles; t += units, ++lt) {
             const int buf = lt & 1;
-            const int m0 = (t / p.tiles_n) * kTileM + static_cast<int>(rank) * kBM, n0 = (t % p.tiles_n) * BN;
+            const Place at = place(t);
+            const int m0 = at.m_tile * kTileM + static_cast<int>(rank) * kBM, n0 = at.n0;
+            // this warp's columns [c_begin, c_end): half of the tile's, or one warp of each
+            // lane quarter takes the 64 of a quarter tile
+            const int cols = kCut && at.cut > 0 ? 64 : kWarpCols;
+            const int c_begin = ((warp - kEpiWarp0) >> 2) * cols, c_end = kCut ? min(c_begin + cols, BN >> at.cut) : c_begin + cols;
             const int y0 = m0 + wq * 32;     // the warp's first row; rows >= m are clipped by TMA
             const bool live = y0 < p.m;      // a box wholly past the last row is not copied
             const float as = as_next;  // 8-bit operands: this row's scale
@@ -461,14 +493,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (kEpi == kAccum) {
                 // fp32 boxes of 32 columns, added into the residual by TMA
 #pragma unroll 1
-                for (int q = 0; q < kWarpCols / 32; ++q) {
-                    const int c = c_begin + 32 * q;
+                for (int c = c_begin; c < c_end; c += 32) {
                     uint32_t acc[32];
                     uint4 braw[4];
                     tmem_ld32(tacc + c, acc);
                     if constexpr (!kInt8) fetch_bias32<T>(bias, n0 + c, braw);
                     tmem_wait_ld();
-                    if (q + 1 == kWarpCols / 32) acc_empty(buf);  // accumulator read out
+                    if (c + 32 == c_end) acc_empty(buf);  // accumulator read out
                     uint32_t w[32];
                     if constexpr (kInt8) {
 #pragma unroll
@@ -498,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float cs[32], sn[32];
                 ok = warp_wait(bar(S::kCsFull), lt & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
                 if (!ok) break;
-                if (n0 + c_begin < p.rope_cols) {
+                if (c_begin < c_end && n0 + c_begin < p.rope_cols) {
                     const int pos0 = m0 % p.seq_len;
                     if (pos0 + kBM <= p.seq_len) {
                         // this row of the staged boxes (16-byte chunk j at j ^ (row & 7))
@@ -525,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 warp_arrive(bar(S::kCsEmpty), lane);  // the rows are in registers
                 const int sw = lane & 7;
 #pragma unroll 1
-                for (int c = c_begin; c < c_begin + kWarpCols; c += 64) {
+                for (int c = c_begin; c < c_end; c += 64) {
                     const bool rot = n0 + c < p.rope_cols;
                     if (lane == 0) bulk_wait_read_all();  // the box's previous head has been copied out
                     __syncwarp();
@@ -584,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
-                    if (c + 64 == c_begin + kWarpCols) acc_empty(buf);
+                    if (c + 64 == c_end) acc_empty(buf);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0 && live && (!kInt8 || n0 + c < p.n)) {
@@ -595,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
                 // kStore: 64-column boxes
 #pragma unroll 1
-                for (int c = c_begin; c < c_begin + kWarpCols; c += 64) {
+                for (int c = c_begin; c < c_end; c += 64) {
                     uint32_t a0[32], a1[32];
                     uint4 b0[4], b1[4];
                     tmem_ld32(tacc + c, a0);
@@ -605,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         fetch_bias32<T>(bias, n0 + c + 32, b1);
                     }
                     tmem_wait_ld();
-                    if (c + 64 == c_begin + kWarpCols) acc_empty(buf);
+                    if (c + 64 == c_end) acc_empty(buf);
                     uint32_t w[32];
                     if constexpr (kInt8) {
 #pragma unroll
@@ -635,6 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+            if (kCut && c_begin >= c_end) acc_empty(buf);  // no columns
             if constexpr (kInt8) warp_arrive(bar(S::kColEmpty), lane);
         }
         // the copies out of the staging boxes have landed before the CTA exits

@@ -216,6 +216,26 @@ def test_linear_int8(cuda_device, m, k, n, dtype):
     _check_linear(got, prod, ref, dtype)
 
 
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("m,n", [(100, 328), (2500, 2056), (2500, 2440), (4101, 2304), (19000, 256), (600, 200)])
+def test_int8_tiles_cut_in_the_last_wave(cuda_device, m, n, pair):
+    """Tiles of 256 columns whose last wave is cut into halves or quarters, in every epilogue: the bits of 64-column tiles."""
+    k = 144
+    x, xs, w, ws, b = _cuda(*_int8_operands(m, k, n, torch.float16, bias=True, seed=m + n))
+    want = F.linear_int8(x, xs, w, ws, b, tile_n=64)
+    assert torch.equal(F.linear_int8(x, xs, w, ws, b, tile_n=256, pair=pair), want)
+    r = torch.randn(m, n, device="cuda")
+    r64, r256 = r.clone(), r.clone()
+    F.accumulate_int8(r64, x, xs, w, ws, tile_n=64)
+    F.accumulate_int8(r256, x, xs, w, ws, tile_n=256, pair=pair)
+    assert torch.equal(r256, r64)
+    if n % 192 == 0:
+        cos, sin = F.rope_tables(m // 3 + 1, "cuda")
+        args = (x, xs, w, ws, b, cos, sin, m // 3 + 1, n // 192)
+        assert torch.equal(F.linear_int8_rope(*args, tile_n=256, pair=pair), F.linear_int8_rope(*args, tile_n=64))
+    F.check_status()
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 768, 264), (8, 256, 72), (40, 144, 328), (300, 1024, 520), (700, 400, 1024)])
 def test_accumulate_int8(cuda_device, m, k, n):
     x, xs, w, ws, b = _int8_operands(m, k, n, torch.float16, bias=True, seed=m)
