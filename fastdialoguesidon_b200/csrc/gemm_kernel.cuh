@@ -412,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 3 && kEpi == kRope) {
         // ------------------------------------------------ cos / sin rows of each tile
-        // (positions (m0 + r) % seq_len, r < 128: one TMA box of each table when
-        // they do not wrap past seq_len; otherwise, or for tiles with no rotated
-        // column, the epilogue reads global memory and the barrier completes empty)
+        // (positions (m0 + r) % seq_len, r < 128: one TMA box of each table when they do
+        // not wrap past seq_len, else copied by the warp; for tiles with no rotated column
+        // the barrier completes empty)
         int lt = 0, armed = -1;
         bool ok = true;
         for (int t = unit0; ok && t < p.tiles; t += units, ++lt) {
@@ -431,12 +431,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive_expect_tx(bar(S::kCsFull), S::kCsBytes);
                     tma_load_2d(sbase + S::cs, &map_cos, bar(S::kCsFull), 0, pos0);
                     tma_load_2d(sbase + S::cs + kBM * 128, &map_sin, bar(S::kCsFull), 0, pos0);
-                } else {
-                    mbar_arrive(bar(S::kCsFull));
                 }
             }
             __syncwarp();
-            if (tma) armed = lt;
+            if (tma) {
+                armed = lt;
+                continue;
+            }
+            if (n0 < p.rope_cols) {  // four rows at a time, 16-byte piece j of a row at j ^ (row & 7)
+#pragma unroll 4
+                for (int r = lane >> 3; r < kBM; r += 4) {
+                    const int64_t from = static_cast<int64_t>((pos0 + r) % p.seq_len) * 64 + 4 * (lane & 7);
+                    const int4 c = __ldg(reinterpret_cast<const int4*>(p.cos_t + from));
+                    const int4 n = __ldg(reinterpret_cast<const int4*>(p.sin_t + from));
+                    const uint32_t to = sbase + S::cs + r * 128 + 16 * ((lane & 7) ^ (r & 7));
+                    st_shared_v4(to, c);
+                    st_shared_v4(to + kBM * 128, n);
+                }
+                fence_proxy_async_smem();  // before the next tile's box lands here
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(bar(S::kCsFull));
         }
         if (!ok && armed >= 0) {  // aborted: the last copies issued land before the CTA exits
             wait_bounded(bar(S::kCsFull), armed & 1, ctl, FDS_STATUS_TIMEOUT_DRAIN, false);
@@ -530,27 +545,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = warp_wait(bar(S::kCsFull), lt & 1, ctl, FDS_STATUS_TIMEOUT_SOFTMAX);
                 if (!ok) break;
                 if (c_begin < c_end && n0 + c_begin < p.rope_cols) {
-                    const int pos0 = m0 % p.seq_len;
-                    if (pos0 + kBM <= p.seq_len) {
-                        // this row of the staged boxes (16-byte chunk j at j ^ (row & 7))
-                        const uint32_t crow = sbase + S::cs + row * 128, srow_s = crow + kBM * 128;
+                    // this row of the staged rows (16-byte chunk j at j ^ (row & 7))
+                    const uint32_t crow = sbase + S::cs + row * 128, srow_s = crow + kBM * 128;
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            const uint32_t off = static_cast<uint32_t>(q ^ (row & 7)) << 4;
-                            const float4 c4 = ld_shared_v4f32(crow + off), s4 = ld_shared_v4f32(srow_s + off);
-                            cs[4 * q] = c4.x, cs[4 * q + 1] = c4.y, cs[4 * q + 2] = c4.z, cs[4 * q + 3] = c4.w;
-                            sn[4 * q] = s4.x, sn[4 * q + 1] = s4.y, sn[4 * q + 2] = s4.z, sn[4 * q + 3] = s4.w;
-                        }
-                    } else {
-                        const int pos = (m0 + row) % p.seq_len;
-                        const float4* cr = reinterpret_cast<const float4*>(p.cos_t + static_cast<int64_t>(pos) * 64);
-                        const float4* sr = reinterpret_cast<const float4*>(p.sin_t + static_cast<int64_t>(pos) * 64);
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) {
-                            const float4 c4 = __ldg(cr + q), s4 = __ldg(sr + q);
-                            cs[4 * q] = c4.x, cs[4 * q + 1] = c4.y, cs[4 * q + 2] = c4.z, cs[4 * q + 3] = c4.w;
-                            sn[4 * q] = s4.x, sn[4 * q + 1] = s4.y, sn[4 * q + 2] = s4.z, sn[4 * q + 3] = s4.w;
-                        }
+                    for (int q = 0; q < 8; ++q) {
+                        const uint32_t off = static_cast<uint32_t>(q ^ (row & 7)) << 4;
+                        const float4 c4 = ld_shared_v4f32(crow + off), s4 = ld_shared_v4f32(srow_s + off);
+                        cs[4 * q] = c4.x, cs[4 * q + 1] = c4.y, cs[4 * q + 2] = c4.z, cs[4 * q + 3] = c4.w;
+                        sn[4 * q] = s4.x, sn[4 * q + 1] = s4.y, sn[4 * q + 2] = s4.z, sn[4 * q + 3] = s4.w;
                     }
                 }
                 warp_arrive(bar(S::kCsEmpty), lane);  // the rows are in registers
