@@ -121,7 +121,9 @@ int max_pairs() {
 // Pieces (log2) that the tiles of the last wave are cut into, so that more SMs share
 // them: as many as fit into one wave. Whole / cut, us: 4101 x 768 -> 2304 10.6 / 9.7,
 // 10000 x 1024 -> 1024 15.3 / 13.6, 2500 x 768 -> 2304 10.1 / 7.9; where nothing is cut
-// the choice costs 1 % (6000 x 1024 -> 3072 19.9 / 20.1).
+// the choice costs 1 % (6000 x 1024 -> 3072 19.9 / 20.1). Not with RoPE, whose pieces
+// would read whole boxes of W (no map left): 2500 x 768 11.8 / 10.7, but 10000 x 1024 ->
+// 3072 33.4 / 35.1.
 int last_cut(int bn, int epilogue, int64_t tiles, int64_t units) {
     const int64_t rest = tiles % units;
     if (bn != 256 || epilogue == FDS_EPILOGUE_ROPE || rest == 0) return 0;

@@ -15,7 +15,7 @@
 // and the epilogues read D[m, n] = sum * (a_scale[m] * w_scale[n]).
 //
 // Persistent CTAs, one per SM at most, walk the output tiles in a static
-// stride: 128 x BN tiles, one per CTA, or (kPair) 256 x BN tiles over a
+// stride (of 8-bit operands the last ones may be cut, fds_int8.cu last_cut): 128 x BN tiles, one per CTA, or (kPair) 256 x BN tiles over a
 // cluster of two CTAs that share each tensor-core operation (tcgen05
 // cta_group::2: each CTA loads its own 128 rows of A and half of the tile's W
 // rows, so a CTA moves 32 KB per 64-deep k-block of a 256-wide tile instead of
@@ -27,7 +27,9 @@
 //               K = 16, fp32 accumulators in TMEM
 //   warp 2      TMEM owner (allocates / releases the 2 x BN columns); 8-bit
 //               operands: the tile's column scales and biases into shared memory
-//   warp 3      RoPE: the tile's cos / sin rows
+//   warp 3      RoPE: the tile's cos / sin rows (a TMA box of each table; tiles that
+//               wrap into the next window copied: read by the epilogue from global
+//               memory instead, 3000 x 768 in windows of 50 rows took 23.3 us, not 16.3)
 //   warps 4-11  epilogue: thread = output row = TMEM lane; two warps per lane
 //               quarter, each taking half of the tile's columns. A warp turns
 //               128 bytes of each of its 32 rows at a time into a swizzled
@@ -538,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // one 64-column head per box (both halves of the rotation).
                 // cos / sin repeat every 32 columns (cat([f, f])): the row's 32
                 // pairs serve every head of the tile, so they are read once per
-                // tile (uncoalesced: a warp's lanes are 32 rows) and kept in
+                // tile and kept in
                 // registers; each 16-pair chunk goes straight into the staging
                 // box, so no whole head row is held
                 float cs[32], sn[32];
