@@ -29,9 +29,9 @@ int make_map(CUtensorMap* map, CUtensorMapDataType type, int esize, const void* 
     return FDS_OK;
 }
 
-template <typename T, int BN, int kEpi, bool kPair>
+template <typename T, int BN, int kEpi, bool kPair, bool kCut = false>
 int launch(const Maps& m, const fds::gemm::Params& p, int grid, cudaStream_t stream) {
-    auto kern = fds::gemm::gemm_kernel<T, BN, kEpi, kPair, true>;
+    auto kern = fds::gemm::gemm_kernel<T, BN, kEpi, kPair, true, kCut>;
     constexpr int smem = fds::gemm::Smem<BN, kPair, kEpi == fds::gemm::kRope, true>::alloc;
     static std::atomic<uint64_t> smem_set{0};
     cudaError_t e = set_smem_once(kern, smem, smem_set);
@@ -46,6 +46,11 @@ int launch(const Maps& m, const fds::gemm::Params& p, int grid, cudaStream_t str
 
 template <typename T, int BN, bool kPair>
 int launch_epi(int epi, const Maps& m, const fds::gemm::Params& p, int grid, cudaStream_t s) {
+    if constexpr (BN == 256) {
+        if (p.cut > 0)
+            return epi == FDS_EPILOGUE_STORE ? launch<T, BN, fds::gemm::kStore, kPair, true>(m, p, grid, s)
+                                             : launch<T, BN, fds::gemm::kAccum, kPair, true>(m, p, grid, s);
+    }
     switch (epi) {
         case FDS_EPILOGUE_STORE: return launch<T, BN, fds::gemm::kStore, kPair>(m, p, grid, s);
         case FDS_EPILOGUE_ROPE: return launch<T, BN, fds::gemm::kRope, kPair>(m, p, grid, s);
@@ -120,10 +125,9 @@ int max_pairs() {
 
 // Pieces (log2) that the tiles of the last wave are cut into, so that more SMs share
 // them: as many as fit into one wave. Whole / cut, us: 4101 x 768 -> 2304 10.6 / 9.7,
-// 10000 x 1024 -> 1024 15.3 / 13.6, 2500 x 768 -> 2304 10.1 / 7.9; where nothing is cut
-// the choice costs 1 % (6000 x 1024 -> 3072 19.9 / 20.1). Not with RoPE, whose pieces
-// would read whole boxes of W (no map left): 2500 x 768 11.8 / 10.7, but 10000 x 1024 ->
-// 3072 33.4 / 35.1.
+// 10000 x 1024 -> 1024 15.3 / 13.6, 2500 x 768 -> 2304 10.1 / 7.9. Not with RoPE, whose
+// pieces would read whole boxes of W (no map left): 2500 x 768 11.8 / 10.7, but 10000 x
+// 1024 -> 3072 33.4 / 35.1.
 int last_cut(int bn, int epilogue, int64_t tiles, int64_t units) {
     const int64_t rest = tiles % units;
     if (bn != 256 || epilogue == FDS_EPILOGUE_ROPE || rest == 0) return 0;

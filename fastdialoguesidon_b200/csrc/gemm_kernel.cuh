@@ -15,7 +15,7 @@
 // and the epilogues read D[m, n] = sum * (a_scale[m] * w_scale[n]).
 //
 // Persistent CTAs, one per SM at most, walk the output tiles in a static
-// stride (of 8-bit operands the last ones may be cut, fds_int8.cu last_cut): 128 x BN tiles, one per CTA, or (kPair) 256 x BN tiles over a
+// stride (kCut: the last ones in pieces, fds_int8.cu last_cut): 128 x BN tiles, one per CTA, or (kPair) 256 x BN tiles over a
 // cluster of two CTAs that share each tensor-core operation (tcgen05
 // cta_group::2: each CTA loads its own 128 rows of A and half of the tile's W
 // rows, so a CTA moves 32 KB per 64-deep k-block of a 256-wide tile instead of
@@ -186,7 +186,10 @@ __device__ __forceinline__ void stage_row(uint32_t srow, int lane, const uint32_
 }
 
 // T: the operand type (of the bias and the 16-bit output, for 8-bit operands).
-template <typename T, int BN, int kEpi, bool kPair, bool kInt8 = false>
+// kCut: the last tiles, where they would fill at most half a wave, come as pieces of
+// fewer columns (8-bit operands, 256-column tiles; a kernel of its own, since the
+// pieces' bounds cost whole tiles 1 %).
+template <typename T, int BN, int kEpi, bool kPair, bool kInt8 = false, bool kCut = false>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_cos,
@@ -212,9 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int kb_n = kInt8 ? (p.k + kBKe - 1) / kBKe : p.k / kBKe;  // 8-bit: the last stage zero-filled past k
-    // The last tiles, where they would fill less than half a wave, as pieces of fewer
-    // columns: tile t's rows, first column and log2 of BN / its columns.
-    constexpr bool kCut = kInt8 && BN == 256 && kEpi != kRope;
+    // tile t's rows, first column and log2 of BN / its columns
+    static_assert(!kCut || (kInt8 && BN == 256 && kEpi != kRope), "which tiles are cut");
     struct Place {
         int m_tile, n0, cut;
     };
