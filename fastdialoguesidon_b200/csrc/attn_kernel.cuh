@@ -722,20 +722,25 @@ struct RowSoftmax {
                 if (c >= lim) s[c] = -INFINITY;
         }
 
+        // (kMaskWindow: a NaN score becomes the maximum, for the polynomial below takes
+        // it for a small one, and a row of nothing else would look like one without keys)
+        constexpr bool kNan = kMask == kMaskWindow;
+        const auto max3 = [](float a, float b, float c) { return kNan ? fmax3_nan(a, b, c) : fmax3(a, b, c); };
+        const auto max2 = [](float a, float b) { return kNan ? fmax_nan(a, b) : fmaxf(a, b); };
         float mx[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) mx[u] = fmax3(s[u], s[8 + u], s[16 + u]);
+        for (int u = 0; u < 8; ++u) mx[u] = max3(s[u], s[8 + u], s[16 + u]);
 #pragma unroll
         for (int c = 24; c < 120; c += 16) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) mx[u] = fmax3(mx[u], s[c + u], s[c + 8 + u]);
+            for (int u = 0; u < 8; ++u) mx[u] = max3(mx[u], s[c + u], s[c + 8 + u]);
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) mx[u] = fmaxf(mx[u], s[120 + u]);
-        const float mxa = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+        for (int u = 0; u < 8; ++u) mx[u] = max2(mx[u], s[120 + u]);
+        const float mxa = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max2(mx[6], mx[7]));
         const float tile_max = fmaf(mxa, mult, cb);
 
-        const bool rescale = tile_max > m_run + kRescaleThreshold;
+        const bool rescale = kNan ? !(tile_max <= m_run + kRescaleThreshold) : tile_max > m_run + kRescaleThreshold;
         float alpha = 1.f;
         if (rescale) {
             alpha = ex2_approx(m_run - tile_max);  // 0 on the item's first tile

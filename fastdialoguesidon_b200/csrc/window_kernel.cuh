@@ -415,7 +415,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) window_tile_kernel(const __gr
                 ok = rs.template step<false, kMaskWindow>(t, 0.f);
             }
             const bool none = rs.m_run == -INFINITY;  // no key seen
-            const float inv = none ? 1.f : 1.f / rs.l_run;
+            // (a score of plus infinity: every weight is NaN, whatever the exponentials made of it)
+            const float inv = none ? 1.f : (rs.m_run < INFINITY ? 1.f / rs.l_run : __uint_as_float(0x7fffffffu));
             uint32_t o[64];
             if (ok && t1 > rs.t_begin) {
                 // (the next unit's first P V overwrites O only after this warpgroup's

@@ -73,8 +73,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     into ``out`` when given. Query i of window b sits at position
     ``p = q_start[b] + i`` (``q_start`` int32 CUDA [B], default 0) and sees key j
     iff ``j < kv_len[b]`` (int32 CUDA [B], default Lk), ``j <= p + right`` and
-    (``j >= p - left`` or ``j < sinks``). A query that sees no key yields zeros.
-    ``scale`` defaults to 1/sqrt(64).
+    (``j >= p - left`` or ``j < sinks``). A query that sees no key, or none whose
+    score is above minus infinity, yields zeros; one with a score that is NaN or
+    plus infinity yields NaN. ``scale`` defaults to 1/sqrt(64).
 
     The tensors may be views: any strides that are multiples of 8 elements with
     contiguous 64-element heads, so ``qkv.view(B, L, 3, H, 64)[:, :, 0]`` of a

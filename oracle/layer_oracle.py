@@ -32,6 +32,31 @@ def window_attention(q, k, v, left, right=0, sinks=0, q_start=None, kv_len=None,
     return out
 
 
+def window_attention_by_head(q, k, v, left, right=0, sinks=0, q_start=None, kv_len=None, scale=0.125):
+    """:func:`window_attention` as one product per window and head, on the tensors'
+    device, for sizes the loop over queries is too slow for. Excluded keys weigh 0,
+    and those that no query of a window sees are dropped."""
+    batch, q_len, heads, dim = q.shape
+    k_len, group, dev = k.shape[1], heads // k.shape[2], q.device
+    out = torch.zeros(batch, q_len, heads, dim, dtype=torch.float64, device=dev)
+    j = torch.arange(k_len, device=dev)
+    for b in range(batch):
+        end = k_len if kv_len is None else min(max(int(kv_len[b]), 0), k_len)
+        p = (0 if q_start is None else int(q_start[b])) + torch.arange(q_len, device=dev)[:, None]
+        seen = (j < end) & (j <= p + right) & ((j >= p - left) | (j < sinks))
+        ids = seen.any(0).nonzero()[:, 0]
+        if len(ids) == 0:
+            continue
+        seen, some = seen[:, ids], seen.any(1)
+        for h in range(heads):
+            s = (q[b, :, h].double() @ k[b, ids, h // group].double().t()) * scale
+            s = torch.where(seen, s, -torch.inf)
+            w = torch.exp(s - torch.where(some, s.amax(1), 0.0)[:, None])
+            o = (w @ v[b, ids, h // group].double()) / w.sum(1, keepdim=True)
+            out[b, :, h] = torch.where(some[:, None], o, 0.0)
+    return out
+
+
 def quantize_rows(x):
     """(int8, fp32 scale) by the operator's definition, in fp32 as it states it."""
     x = x.float()
