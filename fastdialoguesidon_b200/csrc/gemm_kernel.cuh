@@ -167,6 +167,15 @@ __device__ __forceinline__ void scale4(float* y, const uint32_t* acc, float as, 
     y[3] = fmaf(static_cast<float>(static_cast<int32_t>(acc[3])), as * w.w, to_f<T>(bt[3]));
 }
 
+// Rotate-half RoPE of the pair (a, b), columns d and d + 32 of a head: (a c - b s, b c + a s).
+// Which product the sum is fused with is written out, here and in scale4, so that every
+// kernel that computes a result (gemv_i8_kernel.cuh too) rounds it alike.
+__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
+    const float x1 = a, x2 = b;
+    a = fmaf(x1, c, -__fmul_rn(x2, s));
+    b = fmaf(x1, s, __fmul_rn(x2, c));
+}
+
 // This lane's 128-byte row of its warp's staging box (16-byte chunk j at chunk
 // j ^ (row & 7): the tensor map's 128-byte swizzle, and no two lanes of a
 // quarter-warp on the same banks), written once the box's previous contents
@@ -599,11 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         if (rot) {
 #pragma unroll
-                            for (int d = 0; d < 16; ++d) {
-                                const float x1 = a[d], x2 = b[d];
-                                a[d] = x1 * cs[d0 + d] - x2 * sn[d0 + d];
-                                b[d] = x2 * cs[d0 + d] + x1 * sn[d0 + d];
-                            }
+                            for (int d = 0; d < 16; ++d) rotate(a[d], b[d], cs[d0 + d], sn[d0 + d]);
                         }
                         // columns d0 .. d0 + 15 are 16-byte chunks d0 / 8, d0 / 8 + 1 of
                         // the 128-byte row; columns 32 + d0 .. chunks 4 + d0 / 8, ..

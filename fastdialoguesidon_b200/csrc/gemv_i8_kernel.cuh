@@ -101,18 +101,16 @@ __global__ void __launch_bounds__(32 * kWarps) gemv_i8_kernel(const Params p) {
     if (lane >= M || lane >= p.m) return;
     const float as = __ldg(p.a_scale + lane);
     const T* bias = static_cast<const T*>(p.bias);
-    float y0 = static_cast<float>(s0) * (as * __ldg(p.w_scale + r0)) + (bias != nullptr ? gemm::to_f<T>(bias[r0]) : 0.f);
-    float y1 = static_cast<float>(s1) * (as * __ldg(p.w_scale + r1)) + (bias != nullptr ? gemm::to_f<T>(bias[r1]) : 0.f);
+    float y0 = fmaf(static_cast<float>(s0), as * __ldg(p.w_scale + r0), bias != nullptr ? gemm::to_f<T>(bias[r0]) : 0.f);
+    float y1 = fmaf(static_cast<float>(s1), as * __ldg(p.w_scale + r1), bias != nullptr ? gemm::to_f<T>(bias[r1]) : 0.f);
     if constexpr (kEpi == gemm::kAccum) {
         float* o = static_cast<float*>(p.out) + lane * p.out_stride;
-        o[r0] += y0;
-        o[r1] += y1;
+        o[r0] = __fadd_rn(o[r0], y0);
+        o[r1] = __fadd_rn(o[r1], y1);
     } else {
         if (kEpi == gemm::kRope && r0 < p.rope_cols) {
             const int64_t at = static_cast<int64_t>(lane % p.seq_len) * 64 + (r0 & 63);
-            const float c = __ldg(p.cos_t + at), s = __ldg(p.sin_t + at), t = y0;
-            y0 = t * c - y1 * s;
-            y1 = y1 * c + t * s;
+            gemm::rotate(y0, y1, __ldg(p.cos_t + at), __ldg(p.sin_t + at));
         }
         T* o = static_cast<T*>(p.out) + lane * p.out_stride;
         o[r0] = static_cast<T>(y0);
