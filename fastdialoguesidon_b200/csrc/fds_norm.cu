@@ -11,11 +11,20 @@ namespace {
 
 using namespace fds::norm;
 
+// CTAs of `warps` warps that an SM holds at once: 16 warps at 128 registers, and each
+// CTA's ring, reduction slots and the 1 KB that every CTA takes in 228 KB.
+template <int NCH, int R, int kMode, bool kXf32>
+int resident(int warps) {
+    const int bytes = Ring<NCH, kMode, kXf32>::bytes(32 * warps) + kReduceBytes<R> + 1024;
+    return std::max(1, std::min(kMaxWarps / warps, 228 * 1024 / bytes));
+}
+
 template <typename T, int NCH, int R, int kMode, bool kXf32, bool kQuant>
-int launch(Params& p, int threads, int per_sm, int sms, cudaStream_t stream) {
+int launch(Params& p, int warps, int sms, cudaStream_t stream) {
+    using Rg = Ring<NCH, kMode, kXf32>;
+    const int threads = 32 * warps, per_sm = resident<NCH, R, kMode, kXf32>(warps);
     const dim3 grid(static_cast<unsigned>(std::min(p.rows, sms * per_sm))), block(threads);
     auto kern = residual_norm_kernel<T, NCH, R, kMode, kXf32, kQuant>;
-    using Rg = Ring<NCH, kMode, kXf32>;
     static std::atomic<uint64_t> smem_set{0};
     cudaError_t e = set_smem_once(kern, Rg::bytes(32 * kMaxWarps), smem_set);
     if (e != cudaSuccess) return set_error(FDS_ERR_CUDA, "cudaFuncSetAttribute(norm): %s", cudaGetErrorString(e));
@@ -26,19 +35,19 @@ int launch(Params& p, int threads, int per_sm, int sms, cudaStream_t stream) {
 }
 
 // A CTA as wide as the row: 8 columns a thread up to 4096, 16 or 32 beyond. The
-// grid is what the SMs hold at once (16 warps each at 128 registers); four rows at a
-// time once a CTA has two or more (3000 x 768 fp32 stream: 6.9 us against 8.3 us row
-// by row, 6000 x 768: 13.9 against 16.9), single rows below, which are bound by one
-// row's latency.
+// grid is what the SMs hold at once; four rows at a time once a CTA has two or more
+// (3000 x 768 fp32 stream: 6.9 us against 8.3 us row by row, 6000 x 768: 13.9 against
+// 16.9), single rows below, which are bound by one row's latency. (A grid of 16 CTAs
+// an SM where shared memory holds 14 ran a second wave of whole CTAs: 8000 x 256 7.1
+// us against 5.7, 100000 x 128 37.6 against 30.3.)
 template <typename T, int kMode, bool kXf32, bool kQuant>
 int launch_shape(Params& p, int sms, cudaStream_t s) {
     const int nch = p.c <= 4096 ? 1 : (p.c <= 8192 ? 2 : 4);
     const int warps = (p.c + 256 * nch - 1) / (256 * nch);
-    const int per_sm = std::max(1, 16 / warps);
-    if (nch == 4) return launch<T, 4, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
-    if (nch == 2) return launch<T, 2, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
-    if (p.rows >= 2 * sms * per_sm) return launch<T, 1, 4, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
-    return launch<T, 1, 1, kMode, kXf32, kQuant>(p, 32 * warps, per_sm, sms, s);
+    if (nch == 4) return launch<T, 4, 1, kMode, kXf32, kQuant>(p, warps, sms, s);
+    if (nch == 2) return launch<T, 2, 1, kMode, kXf32, kQuant>(p, warps, sms, s);
+    if (p.rows >= 2 * sms * resident<1, 4, kMode, kXf32>(warps)) return launch<T, 1, 4, kMode, kXf32, kQuant>(p, warps, sms, s);
+    return launch<T, 1, 1, kMode, kXf32, kQuant>(p, warps, sms, s);
 }
 
 template <typename T, int NCH, int kR>

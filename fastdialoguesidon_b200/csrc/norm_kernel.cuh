@@ -156,6 +156,8 @@ struct MaxBits {
 
 constexpr int kSlots = 5;       // reductions per group of rows at most
 constexpr int kMaxWarps = 16;
+template <int R>
+constexpr int kReduceBytes = 2 * kSlots * kMaxWarps * R * 4;  // two sets of slots, used in turn
 
 // Reduces v[r] (row r) over the CTA's threads, in place. Four rows share their
 // shuffles: after two exchanging steps each 8-lane group holds one row. `red`
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) residual_norm_kernel(const 
     using Rg = Ring<NCH, kMode, kXf32>;
     constexpr bool kKeep = NCH < 4;  // coefficients in registers; the widest rows read them again per group
     static_assert((Rg::kRows & (Rg::kRows - 1)) == 0 && Rg::kRows >= R, "ring rows");
-    __shared__ __align__(16) float red_all[2 * kSlots * kMaxWarps * R];
+    __shared__ __align__(16) float red_all[kReduceBytes<R> / 4];
     extern __shared__ __align__(16) uint8_t ring_raw[];
     grid_launch_dependents();
     grid_dependency_wait();
