@@ -142,10 +142,7 @@ extern "C" int fds_residual_norm_fwd(const FdsResidualNormArgs* a, void* stream)
     p.x_f32 = a->x_f32, p.param_f32 = a->param_f32, p.post = a->post, p.norm = a->norm;
     p.alpha = a->alpha, p.eps = a->eps;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const auto wide = [&](const void* q, int64_t stride) {
-        return (reinterpret_cast<uintptr_t>(q) & 31u) == 0 && (p.rows <= 1 || stride % 8 == 0);
-    };
-    p.x_wide = wide(p.x, p.x_stride) && wide(p.x_out, p.x_out_stride);
+    p.x_out_wide = (reinterpret_cast<uintptr_t>(p.x_out) & 31u) == 0 && (p.rows <= 1 || p.x_out_stride % 8 == 0);
     const int sms = sm_count();
     if (sms <= 0) return set_error(FDS_ERR_CUDA, "cannot query the SM count of the current device");
     const int rc = a->dtype == FDS_DTYPE_FP16 ? launch_type<__half>(p, sms, s) : launch_type<__nv_bfloat16>(p, sms, s);

@@ -62,7 +62,7 @@ struct Params {
     int64_t gate_stride, mod_stride;                     // elements between windows (0: shared)
     int32_t rows, c, length;  // rows per window
     int32_t x_f32, param_f32;
-    int32_t x_wide;           // fp32 rows of x and x_out on 32-byte boundaries: 256-bit accesses
+    int32_t x_out_wide;       // fp32 rows of x_out on 32-byte boundaries: 256-bit stores
     int32_t post, norm;       // Kind
     float alpha, eps;
 };
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) residual_norm_kernel(const 
                     const float(&o)[8] = x[r][i];
                     char* to = ox + r * ox_step + static_cast<int64_t>(8 * i) * blockDim.x * (kXf32 ? 4 : 2);
                     if constexpr (kXf32)
-                        store8(reinterpret_cast<float*>(to), p.x_wide != 0, o);
+                        store8(reinterpret_cast<float*>(to), p.x_out_wide != 0, o);
                     else
                         *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]),
                                                                    pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));

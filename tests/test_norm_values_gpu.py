@@ -69,6 +69,21 @@ def test_norm_without_a_block_many_groups_of_rows(cuda_device, c, stream):
     assert bool(((q.double() * s - rh).abs() <= s / 2 + 2.0 ** -17 * big * 2 + 4 * V * 127 * s).all())
 
 
+@pytest.mark.parametrize("off_x,off_out", [(0, 0), (4, 0), (0, 4), (4, 4)])
+@pytest.mark.parametrize("rows", [1, 50, 4000])
+def test_residual_norm_stream_alignments(cuda_device, off_x, off_out, rows):
+    """fp32 rows on 16- or 32-byte boundaries, on either side: the same bits, and what lies beside them stays."""
+    g = torch.Generator().manual_seed(rows)
+    x, y = torch.randn(rows, 512, generator=g).cuda(), torch.randn(rows, 512, generator=g).half().cuda()
+    want, h = F.residual_norm(x, y, residual_out=torch.empty_like(x))
+    wide, keep = torch.randn(rows, 520, device="cuda"), torch.zeros(rows, 520, device="cuda")
+    wide[:, off_x:off_x + 512] = x
+    x1, h1 = F.residual_norm(wide[:, off_x:off_x + 512], y, residual_out=keep[:, off_out:off_out + 512])
+    assert torch.equal(x1, want) and torch.equal(h1, h)
+    keep[:, off_out:off_out + 512] = 0
+    assert float(keep.abs().max()) == 0.0
+
+
 @pytest.mark.parametrize("c", [248, 264, 512, 520, 776, 1032, 1544, 2056, 3000, 4088, 8192, 8200])
 @pytest.mark.parametrize("rows", [1, 7, 1001])
 def test_quantize_rows_widths(cuda_device, c, rows):
