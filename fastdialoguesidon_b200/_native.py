@@ -273,7 +273,7 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         if not path.exists():
             if not build_if_missing:
                 raise RuntimeError(f"native library {path} is missing; run fastdialoguesidon_b200.build.build()")
-            _build.build()
+            _build.build_library()
         lib = ctypes.CDLL(str(path))
         lib.fds_flexrel_attn_fwd.argtypes = [ctypes.POINTER(FdsFlexRelArgs), ctypes.c_void_p]
         lib.fds_flexrel_attn_fwd.restype = ctypes.c_int

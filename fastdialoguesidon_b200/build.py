@@ -5,11 +5,13 @@ The library: nvcc, sm_100a only (``-gencode arch=compute_100a,code=sm_100a``),
 static cudart, no torch headers: a plain C ABI (``include/fds_b200.h``) that any
 FFI can load. The extension (``csrc/torch_shim.cpp``, g++, torch's headers)
 checks the layer ops' tensors and calls that ABI. Both live inside the package
-directory so that they travel with the source tree.
+directory so that they travel with the source tree. ``python
+fastdialoguesidon_b200/build.py`` builds the library where torch is not installed.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -49,18 +51,28 @@ def nvcc_path() -> str:
     return cand
 
 
-def _inputs() -> list[Path]:
-    files = [CSRC / s for s in (*SOURCES, SHIM_SOURCE)]
+def _newer(inputs: list[Path], output: Path) -> bool:
+    """``output`` is missing, or older than one of ``inputs``."""
+    return not output.exists() or any(f.stat().st_mtime > output.stat().st_mtime for f in inputs)
+
+
+def _library_stale() -> bool:
+    files = [CSRC / s for s in SOURCES]
     files += sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
     files += sorted(INCLUDE_DIR.glob("*.h"))
-    return files
+    return _newer(files, LIB_PATH)
+
+
+def _extension_stale() -> bool:
+    return _has_torch() and _newer([CSRC / SHIM_SOURCE, *sorted(INCLUDE_DIR.glob("*.h"))], SHIM_PATH)
+
+
+def _has_torch() -> bool:
+    return importlib.util.find_spec("torch") is not None
 
 
 def is_stale() -> bool:
-    if not (LIB_PATH.exists() and SHIM_PATH.exists()):
-        return True
-    mtime = min(LIB_PATH.stat().st_mtime, SHIM_PATH.stat().st_mtime)
-    return any(f.stat().st_mtime > mtime for f in _inputs())
+    return _library_stale() or _extension_stale()
 
 
 def _run(cmd: list[str], verbose: bool) -> str:
@@ -68,13 +80,24 @@ def _run(cmd: list[str], verbose: bool) -> str:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     return res.stdout + res.stderr
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library and the extension if any source is newer (or ``force``)."""
-    if not force and not is_stale():
+    """Compile the library and the extension, each if a source of its own is newer
+    (or ``force``). The library is in place whatever becomes of the extension, which
+    a tree without torch has no use for."""
+    with ThreadPoolExecutor(max_workers=1) as pool:  # side by side
+        extension = pool.submit(build_extension, force, verbose) if _has_torch() else None
+        build_library(force, verbose)
+        if extension is not None:
+            extension.result()
+    return LIB_PATH
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    if not (force or _library_stale()):
         return LIB_PATH
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     # the sources compile side by side, each to an object, then link
@@ -85,14 +108,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return _run([nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xptxas=-v", "-Xcompiler",
                      "-fPIC,-fvisibility=hidden", "-I", str(INCLUDE_DIR), "-c", "-o", str(obj), str(CSRC / src)], verbose)
 
-    with ThreadPoolExecutor(max_workers=min(len(SOURCES) + 1, os.cpu_count() or 1)) as pool:
-        shim = pool.submit(_build_shim, verbose)
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
         log = "".join(pool.map(compile_one, zip(SOURCES, objs)))
     tmp = LIB_PATH.with_suffix(".so.tmp")
     _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(tmp), *map(str, objs)], verbose)
     for obj in objs:
         obj.unlink()
-    shim.result()
     if verbose:
         sys.stdout.write(log)
     check_launch_registers(log)
@@ -100,7 +121,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB_PATH
 
 
-def _build_shim(verbose: bool) -> None:
+def build_extension(force: bool = False, verbose: bool = False) -> Path:
+    if not (force or _extension_stale()):
+        return SHIM_PATH
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
     import sysconfig
 
     import torch
@@ -115,6 +139,7 @@ def _build_shim(verbose: bool) -> None:
           str(CSRC / SHIM_SOURCE), "-o", str(tmp), "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
           "-lc10_cuda"], verbose)
     os.replace(tmp, SHIM_PATH)
+    return SHIM_PATH
 
 
 def check_launch_registers(ptxas_log: str) -> None:

@@ -48,7 +48,7 @@ def _load():
         if _ext is None:
             lib = N.load()
             if not _build.SHIM_PATH.exists():
-                _build.build(force=True)
+                _build.build_extension()
             spec = importlib.util.spec_from_file_location("_fds_torch", _build.SHIM_PATH)
             ext = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(ext)
