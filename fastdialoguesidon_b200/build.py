@@ -11,12 +11,15 @@ fastdialoguesidon_b200/build.py`` builds the library where torch is not installe
 
 from __future__ import annotations
 
+import fcntl
 import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
+from contextlib import contextmanager
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -87,7 +90,8 @@ def _run(cmd: list[str], verbose: bool) -> str:
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the library and the extension, each if a source of its own is newer
     (or ``force``). The library is in place whatever becomes of the extension, which
-    a tree without torch has no use for."""
+    a tree without torch has no use for. Processes that build at once do so in turn,
+    and the later ones find what the first has built."""
     with ThreadPoolExecutor(max_workers=1) as pool:  # side by side
         extension = pool.submit(build_extension, force, verbose) if _has_torch() else None
         build_library(force, verbose)
@@ -96,49 +100,62 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB_PATH
 
 
+@contextmanager
+def _workspace(output: Path):
+    """A directory of this process's own beside ``output``, while no other process
+    builds ``output``."""
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    with open(LIB_DIR / f".{output.name}.lock", "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        with tempfile.TemporaryDirectory(dir=LIB_DIR, prefix=".build-") as tmp:
+            yield Path(tmp)
+
+
 def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not (force or _library_stale()):
         return LIB_PATH
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    # the sources compile side by side, each to an object, then link
-    objs = [LIB_DIR / (Path(src).stem + ".o") for src in SOURCES]
+    with _workspace(LIB_PATH) as work:
+        if not (force or _library_stale()):  # built while this process waited
+            return LIB_PATH
+        # the sources compile side by side, each to an object, then link
+        objs = [work / (Path(src).stem + ".o") for src in SOURCES]
 
-    def compile_one(job: tuple[str, Path]) -> str:
-        src, obj = job
-        return _run([nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xptxas=-v", "-Xcompiler",
-                     "-fPIC,-fvisibility=hidden", "-I", str(INCLUDE_DIR), "-c", "-o", str(obj), str(CSRC / src)], verbose)
+        def compile_one(job: tuple[str, Path]) -> str:
+            src, obj = job
+            return _run([nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xptxas=-v", "-Xcompiler",
+                         "-fPIC,-fvisibility=hidden", "-I", str(INCLUDE_DIR), "-c", "-o", str(obj), str(CSRC / src)], verbose)
 
-    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
-        log = "".join(pool.map(compile_one, zip(SOURCES, objs)))
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(tmp), *map(str, objs)], verbose)
-    for obj in objs:
-        obj.unlink()
-    if verbose:
-        sys.stdout.write(log)
-    check_launch_registers(log)
-    os.replace(tmp, LIB_PATH)
+        with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+            log = "".join(pool.map(compile_one, zip(SOURCES, objs)))
+        linked = work / LIB_PATH.name
+        _run([nvcc_path(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", str(linked), *map(str, objs)], verbose)
+        if verbose:
+            sys.stdout.write(log)
+        check_launch_registers(log)
+        os.replace(linked, LIB_PATH)
     return LIB_PATH
 
 
 def build_extension(force: bool = False, verbose: bool = False) -> Path:
     if not (force or _extension_stale()):
         return SHIM_PATH
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
     import sysconfig
 
     import torch
 
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc_path()).resolve().parents[1]
-    tmp = SHIM_PATH.with_suffix(".so.tmp")
-    _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          "-I", str(INCLUDE_DIR), "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
-          "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
-          str(CSRC / SHIM_SOURCE), "-o", str(tmp), "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
-          "-lc10_cuda"], verbose)
-    os.replace(tmp, SHIM_PATH)
+    with _workspace(SHIM_PATH) as work:
+        if not (force or _extension_stale()):
+            return SHIM_PATH
+        linked = work / SHIM_PATH.name
+        _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+              "-I", str(INCLUDE_DIR), "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+              "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
+              str(CSRC / SHIM_SOURCE), "-o", str(linked), "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+              "-lc10_cuda"], verbose)
+        os.replace(linked, SHIM_PATH)
     return SHIM_PATH
 
 

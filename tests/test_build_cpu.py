@@ -63,7 +63,7 @@ def _run(tree, code="", args=()):
 
 
 def _built(tree):
-    return sorted(p.name for p in (tree / "fastdialoguesidon_b200" / "_lib").iterdir())
+    return sorted(p.name for p in (tree / "fastdialoguesidon_b200" / "_lib").iterdir() if not p.name.endswith(".lock"))
 
 
 def test_both_are_built(tree):
@@ -86,6 +86,22 @@ def test_the_library_stays_when_the_extension_fails(tree):
     rc, out = _run(tree)
     assert rc != 0 and "g++ failed" in out and "no such compiler" in out, out
     assert LIBRARY in _built(tree)
+
+
+def test_processes_that_build_at_once(tree):
+    """Four, on a fresh tree, each step of which takes a while: one builds, every one
+    succeeds, and nothing but the results is left."""
+    _tool(tree, "nvcc", NVCC.replace("out=; srcs=", "out=; srcs=; echo call >> calls; sleep 0.2"))
+    procs = [_start(tree, "sys.modules['torch'] = None") for _ in range(4)]
+    outs = [(p.communicate(timeout=120)[0], p.returncode) for p in procs]
+    assert all(rc == 0 for _, rc in outs), outs
+    assert _built(tree) == [LIBRARY]
+    assert len((tree / "calls").read_text().split()) == 6  # five sources and a link
+    procs = [_start(tree, "sys.modules['torch'] = None", ["--force"]) for _ in range(3)]
+    outs = [(p.communicate(timeout=120)[0], p.returncode) for p in procs]
+    assert all(rc == 0 for _, rc in outs), outs
+    text = (tree / "fastdialoguesidon_b200" / "_lib" / LIBRARY).read_text()
+    assert _built(tree) == [LIBRARY] and text.count(".cu") == 5
 
 
 def test_nothing_is_replaced_by_a_library_with_other_registers(tree):
