@@ -1,5 +1,5 @@
 """Build recipe for the in-tree native library ``_lib/libfds_b200.so`` and the
-Python extension ``_lib/_fds_torch.so``.
+Python extension ``_lib/_fds_torch.<python>-torch<version>.so``.
 
 The library: nvcc, sm_100a only (``-gencode arch=compute_100a,code=sm_100a``),
 static cudart, no torch headers: a plain C ABI (``include/fds_b200.h``) that any
@@ -27,7 +27,6 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libfds_b200.so"
-SHIM_PATH = LIB_DIR / "_fds_torch.so"
 INCLUDE_DIR = REPO_DIR / "include"
 
 SHIM_SOURCE = "torch_shim.cpp"
@@ -54,6 +53,14 @@ def nvcc_path() -> str:
     return cand
 
 
+def extension_path() -> Path:
+    """The extension of this Python and this torch: it is bound to the ABI of both, so another
+    version's is another file."""
+    import torch
+
+    return LIB_DIR / f"_fds_torch.{sys.implementation.cache_tag}-torch{torch.__version__}.so"
+
+
 def _newer(inputs: list[Path], output: Path) -> bool:
     """``output`` is missing, or older than one of ``inputs``."""
     return not output.exists() or any(f.stat().st_mtime > output.stat().st_mtime for f in inputs)
@@ -67,7 +74,7 @@ def _library_stale() -> bool:
 
 
 def _extension_stale() -> bool:
-    return _has_torch() and _newer([CSRC / SHIM_SOURCE, *sorted(INCLUDE_DIR.glob("*.h"))], SHIM_PATH)
+    return _has_torch() and _newer([CSRC / SHIM_SOURCE, *sorted(INCLUDE_DIR.glob("*.h"))], extension_path())
 
 
 def _has_torch() -> bool:
@@ -137,26 +144,27 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_extension(force: bool = False, verbose: bool = False) -> Path:
+    path = extension_path()
     if not (force or _extension_stale()):
-        return SHIM_PATH
+        return path
     import sysconfig
 
     import torch
 
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc_path()).resolve().parents[1]
-    with _workspace(SHIM_PATH) as work:
+    with _workspace(path) as work:
         if not (force or _extension_stale()):
-            return SHIM_PATH
-        linked = work / SHIM_PATH.name
+            return path
+        linked = work / path.name
         _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
               "-I", str(INCLUDE_DIR), "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
               "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
               str(CSRC / SHIM_SOURCE), "-o", str(linked), "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
               "-lc10_cuda"], verbose)
-        os.replace(linked, SHIM_PATH)
-    return SHIM_PATH
+        os.replace(linked, path)
+    return path
 
 
 def check_launch_registers(ptxas_log: str) -> None:

@@ -47,9 +47,10 @@ def _load():
     with _lock:
         if _ext is None:
             lib = N.load()
-            if not _build.SHIM_PATH.exists():
+            path = _build.extension_path()
+            if not path.exists():
                 _build.build_extension()
-            spec = importlib.util.spec_from_file_location("_fds_torch", _build.SHIM_PATH)
+            spec = importlib.util.spec_from_file_location("_fds_torch", path)
             ext = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(ext)
             ext.bind(FdsError, _status_addresses, lambda i: _raise_if_timed_out(torch.device("cuda", i)),

@@ -88,6 +88,18 @@ def test_the_library_stays_when_the_extension_fails(tree):
     assert LIBRARY in _built(tree)
 
 
+def test_an_extension_of_another_torch_is_not_taken(tree):
+    """The extension is built again for the torch (or Python) that is there, whatever the files' times."""
+    assert _run(tree)[0] == 0
+    before = _built(tree)
+    rc, out = _run(tree, "import torch; torch.__version__ = '99.1'")
+    assert rc == 0, out
+    new = set(_built(tree)) - set(before)
+    assert len(new) == 1 and "99.1" in new.pop()
+    rc, out = _run(tree, "sys.implementation.cache_tag = 'cpython-399'")
+    assert rc == 0 and any("cpython-399" in n for n in _built(tree)), out
+
+
 def test_processes_that_build_at_once(tree):
     """Four, on a fresh tree, each step of which takes a while: one builds, every one
     succeeds, and nothing but the results is left."""
