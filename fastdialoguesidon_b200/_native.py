@@ -275,6 +275,11 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
                 raise RuntimeError(f"native library {path} is missing; run fastdialoguesidon_b200.build.build()")
             _build.build_library()
         lib = ctypes.CDLL(str(path))
+        # before any other symbol: an older library lacks some
+        lib.fds_abi_version.argtypes = []
+        lib.fds_abi_version.restype = ctypes.c_int
+        if lib.fds_abi_version() != ABI_VERSION:
+            raise RuntimeError(f"{path}: ABI version {lib.fds_abi_version()} != {ABI_VERSION}")
         lib.fds_flexrel_attn_fwd.argtypes = [ctypes.POINTER(FdsFlexRelArgs), ctypes.c_void_p]
         lib.fds_flexrel_attn_fwd.restype = ctypes.c_int
         lib.fds_rope_attn_fwd.argtypes = [ctypes.POINTER(FdsRopeArgs), ctypes.c_void_p]
@@ -296,8 +301,6 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
         ]
         lib.fds_rope_split.restype = ctypes.c_int
-        lib.fds_abi_version.argtypes = []
-        lib.fds_abi_version.restype = ctypes.c_int
         lib.fds_last_error.argtypes = []
         lib.fds_last_error.restype = ctypes.c_char_p
         lib.fds_attn_smem_bytes.argtypes = []
@@ -307,8 +310,6 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fds_attn_schedule.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                           ctypes.c_int64, ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)]
         lib.fds_attn_schedule.restype = ctypes.c_int
-        if lib.fds_abi_version() != ABI_VERSION:
-            raise RuntimeError(f"{path}: ABI version {lib.fds_abi_version()} != {ABI_VERSION}")
         _lib = lib
         return lib
 

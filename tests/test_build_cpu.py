@@ -121,3 +121,17 @@ def test_nothing_is_replaced_by_a_library_with_other_registers(tree):
     rc, out = _run(tree)
     assert rc != 0 and "126 registers" in out, out
     assert LIBRARY not in _built(tree)
+
+
+def test_a_library_of_another_abi_is_refused(tmp_path, monkeypatch):
+    """By its version, although it lacks entry points of this one."""
+    from fastdialoguesidon_b200 import _native as N
+
+    src = tmp_path / "old.c"
+    src.write_text("int fds_abi_version(void) { return 4; }\nint fds_linear_fwd(void *a, void *s) { return 0; }\n")
+    lib = tmp_path / "libold.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(lib), str(src)], check=True)
+    monkeypatch.setattr(N, "_lib", None)
+    monkeypatch.setattr(N._build, "LIB_PATH", lib)
+    with pytest.raises(RuntimeError, match="ABI version 4"):
+        N.load()
