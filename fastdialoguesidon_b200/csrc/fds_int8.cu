@@ -256,6 +256,7 @@ extern "C" int fds_linear_int8_fwd(const FdsLinearInt8Args* a, void* stream) {
     const int64_t units = t.pair ? pairs : sms;
     const int cut = last_cut(t.bn, a->epilogue, tiles, units);
     maps.cos = maps.sin = maps.out;
+    // (the cut tiles' quarter boxes of W travel in the place of the cosines)
     if (cut > 0 && (rc = make_map(&maps.cos, u8, 1, a->w, a->k, a->n, a->w_row_stride, fds::gemm::kRowBytes, t.bn / (t.pair ? 8 : 4))) != FDS_OK)
         return rc;
     if (a->epilogue == FDS_EPILOGUE_ROPE &&

@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kb_n = kInt8 ? (p.k + kBKe - 1) / kBKe : p.k / kBKe;  // 8-bit: the last stage zero-filled past k
     // tile t's rows, first column and log2 of BN / its columns
     static_assert(!kCut || (kInt8 && BN == 256 && kEpi != kRope), "which tiles are cut");
+    const CUtensorMap* const map_w_quarter = &map_cos;  // kCut: in the place of the cosines, which only kRope reads
     struct Place {
         int m_tile, n0, cut;
     };
@@ -294,15 +295,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int m0 = at.m_tile * kTileM + static_cast<int>(rank) * kBM;
             const int n0 = at.n0 + static_cast<int>(rank) * (S::kBNc >> at.cut);
             const uint32_t bytes = S::a_bytes + (S::b_bytes >> at.cut);
-            // the W rows: one box, those of a piece in quarter boxes (the map that the RoPE
-            // epilogue has for its cosines)
+            // the W rows: one box, those of a piece in quarter boxes
             const auto load_w = [&](int st, int kb, auto load) {
                 const uint32_t to = sbase + S::b + st * S::b_bytes;
                 if (!kCut || at.cut == 0) {
                     load(to, &map_b, kb * kBKe, n0);
                 } else {
                     for (int j = 0; j < (4 >> at.cut); ++j)
-                        load(to + j * (S::b_bytes / 4), &map_cos, kb * kBKe, n0 + j * (S::kBNc / 4));
+                        load(to + j * (S::b_bytes / 4), map_w_quarter, kb * kBKe, n0 + j * (S::kBNc / 4));
                 }
             };
             for (int kb = 0; kb < kb_n; ++kb, ++g) {
@@ -583,13 +583,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_ld16(tacc + c + 32 + d0, hi);
                         if constexpr (!kInt8) {
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            bl[q] = bias != nullptr ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + d0) + q)
-                                                    : make_uint4(0, 0, 0, 0);
-                            bh[q] = bias != nullptr
-                                        ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + 32 + d0) + q)
-                                        : make_uint4(0, 0, 0, 0);
-                        }
+                            for (int q = 0; q < 2; ++q) {
+                                bl[q] = bias != nullptr ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + d0) + q)
+                                                        : make_uint4(0, 0, 0, 0);
+                                bh[q] = bias != nullptr
+                                            ? __ldg(reinterpret_cast<const uint4*>(bias + n0 + c + 32 + d0) + q)
+                                            : make_uint4(0, 0, 0, 0);
+                            }
                         }
                         tmem_wait_ld();
                         float a[16], b[16];
@@ -600,11 +600,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 scale4<T>(a + d, lo + d, as, cscale + 4u * at, cbias + 2u * at);
                                 scale4<T>(b + d, hi + d, as, cscale + 4u * at + 128, cbias + 2u * at + 64);
                             }
-                        } else
+                        } else {
 #pragma unroll
-                        for (int d = 0; d < 16; ++d) {
-                            a[d] = round_t<T>(__uint_as_float(lo[d]) + to_f<T>(reinterpret_cast<const T*>(bl)[d]));
-                            b[d] = round_t<T>(__uint_as_float(hi[d]) + to_f<T>(reinterpret_cast<const T*>(bh)[d]));
+                            for (int d = 0; d < 16; ++d) {
+                                a[d] = round_t<T>(__uint_as_float(lo[d]) + to_f<T>(reinterpret_cast<const T*>(bl)[d]));
+                                b[d] = round_t<T>(__uint_as_float(hi[d]) + to_f<T>(reinterpret_cast<const T*>(bh)[d]));
+                            }
                         }
                         if (rot) {
 #pragma unroll
