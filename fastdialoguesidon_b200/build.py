@@ -41,7 +41,7 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # refuses to produce a library in that case.
 ATTN_KERNEL_MARK = "attn_fwd_kernel"
 ATTN_LAUNCH_REGS = 168
-# ... and of the window kernel (csrc/window_kernel.cuh: 128 threads at 208, 128 at 48)
+# ... and of the window kernel (csrc/window_kernel.cuh: 128 threads at 200, 128 at 56)
 WINDOW_KERNEL_MARK = "window_tile_kernel"
 WINDOW_LAUNCH_REGS = 128
 

@@ -29,7 +29,8 @@
 //   Bound by the latency of a softmax warp's own instructions, two warps a
 //   scheduler: 12 heads x 6000 queries x 1000 keys 39.5 us (issue slots 43 %,
 //   exponential units 30 %, DRAM 8 %), 16 x 30000 x 1000 207 us, 597 TFLOP/s over
-//   the pairs seen. A tile of a CTA takes 2250 to 2650 cycles, one with masks 3000;
+//   the pairs seen at full clock (228 us once the power cap holds the SMs at 1.78
+//   GHz). A tile of a CTA takes 2250 to 2650 cycles, one with masks 3000;
 //   from a unit's last tile to the next one's scores another 2200.
 // * window_step_kernel: up to 16 query rows per key head (a decoding step):
 //   bound by reading the keys and values once. Each warp streams its share of the
@@ -39,6 +40,16 @@
 //   4 warps of up to 8 CTAs of a cluster -- are merged the same way. 16 windows x
 //   4 key heads x 4112 keys: 14.6 us, 4.6 TB/s; one window, 12 heads x 1004 keys:
 //   3.7, 1.9 of which an empty launch takes.
+//
+// Scores, maxima, sums, O and the parts' merge are fp32. The weights are rounded to
+// the operand type for the P V product, in both kernels: the tensor cores take P in
+// V's type (fp32 weights would need V as tf32, at half the rate and twice the
+// shared memory), and a rounding of u relative per weight averages out over the
+// keys, below the output's own rounding. Sums are of the unrounded weights. Tiles
+// take 3 in 10 exponentials from a polynomial within 7.5e-5 (attn_kernel.cuh
+// poly_pair), below u / 6 in fp16. In all the error against 64 bits is 1.2 to 1.4
+// times the output's rounding alone (fp16 2.6e-4 to 2.9e-4 against 2.1e-4, bf16
+// 2.1e-3 to 2.3e-3 against 1.7e-3, relative, in the 2-norm).
 //
 // Keys and values that no row of a unit sees may hold anything (a cache's
 // unwritten rows): their scores are replaced, and their value rows are zeroed

@@ -547,7 +547,9 @@ def linear_rope(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, cos: t
     """The DiT's QKV projection with RoPE in its epilogue: ``F.linear(x, w, b)``
     (rounded to x's dtype) followed by ``rope_split``'s rotation of the q and k
     column blocks (position = row % length), written as one [M, 3*heads*64]
-    tensor that :func:`rotated_attention` reads directly. Replaces
+    tensor that :func:`rotated_attention` reads directly. The two 32-column halves
+    of ``cos`` and ``sin`` are equal, as :func:`rope_tables` builds them: only the
+    first is read. Replaces
     triton/src/fds_triton/model.py:318-319 (linear + K.rope_split)."""
     n = w.shape[0]
     _check(n == 3 * heads * HEAD_DIM, lambda: f"w must have 3*heads*64 = {3 * heads * HEAD_DIM} rows (got {n})")
